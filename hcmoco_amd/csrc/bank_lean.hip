@@ -6,7 +6,8 @@
 // Why it exists (r04, profiles/r04_bf16_variants.txt): the bf16 pass is bound by instruction issue, not by
 // bytes in flight -- a 256-byte row costs the same bookkeeping as a 512-byte one.  One ring slot (four rows x three
 // banks per wave) of the general kernel executes ~270 instructions; the same work here takes ~150:
-//   * every product / sum is written on v2f (v_pk_mul_f32 / v_pk_fma_f32) with ONE pairing throughout -- a 32-bit word of
+//   * every product / sum is written on v2f with ONE pairing throughout (two scalar instructions a pair since the packed fp32
+//     forms are switched off in the Makefile; the instruction counts below are those of the packed build) -- a 32-bit word of
 //     a bf16 row unpacks to the pair (w << 16, w & 0xffff0000) = two adjacent columns, the queries and accumulators are
 //     paired the same way -- so no register moves re-pair operands (the vectoriser's pairing differed between the dot
 //     products and the accumulation: ~45 v_mov per slot).  The file is compiled with -fno-slp-vectorize: the 24 DPP row

@@ -38,8 +38,9 @@ __device__ __forceinline__ float sqdist(float ax, float ay, float az, float bx, 
   if (FMA) return fmaf(dz, dz, fmaf(dx, dx, dy * dy));
   return (dx * dx + dy * dy) + dz * dz;
 }
-// Two squared distances at once (two unknown points against one known point) on the packed fp32 lanes
-// (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): element-wise IEEE operations, so each half is bit-identical to sqdist.
+// Two squared distances at once (two unknown points against one known point), written on float pairs:
+// element-wise IEEE operations, so each half is bit-identical to sqdist (two scalar instructions a pair: the Makefile switches the
+// packed fp32 forms off).
 typedef float v2f __attribute__((ext_vector_type(2)));
 template <bool FMA>
 __device__ __forceinline__ v2f sqdist2(v2f ax, v2f ay, v2f az, float bx, float by, float bz) {
@@ -612,7 +613,8 @@ __global__ __launch_bounds__(1024) void fps_generic_kernel(int n, int m, int bs,
 // walks the same chain (profiles/r04_fps_counters.txt: 220 instructions per wave and round = half of the round,
 // most of the rest at the LDS exchange; n = 256 costs 0.4 us a round, n = 4096 0.72) -- so the round is written for
 // the LENGTH of that chain:
-//   * two points per packed instruction (v_pk_add / v_pk_mul / v_pk_fma: element-wise IEEE, bit-identical);
+//   * two points per float pair (element-wise IEEE, bit-identical; the counters above are of the packed fp32 build, which the
+//     Makefile has switched off since);
 //   * running minima are kept as BIT PATTERNS and compared as unsigned integers (distances are >= +0, where the two
 //     orders agree): v_min_u32 / v_max3_u32 need no canonicalising v_max_f32 x, x in front of them and the DPP steps
 //     fuse into v_max_u32_dpp.  Empty slots (k >= n) carry the minimum 0 and the key 0: they never raise a
