@@ -135,6 +135,14 @@ SIGNATURES = {
     'hcm_project_rows_backward': (_i, [_p] * 7 + [_i] * 4 + [Branches, Branches, _p, _i] + [_p] * 5 + [_sz, _p]),
     'hcm_alias_draw_checked': (_i, [_p, _p, _i64, _p, _i, _i, _u64, _u64, _p, _p, _p]),
     'hcm_bank_update_checked': (_i, [_p, _p, _p, _i64, _p, _p, _p, _i64, _p, _i, _i, _f, _p, _p]),
+    'hcm_act8_pitch': (_i64, [_i64]),
+    'hcm_act8_scale_pitch': (_i64, [_i64]),
+    'hcm_act8_pack': (_i, [_p, _i, _i64, _i, _i64, _p, _i64, _p, _i64, _p]),
+    'hcm_act8_unpack': (_i, [_p, _i64, _p, _i64, _i64, _i, _p, _i, _p]),
+    'hcm_fp8_weight_pack': (_i, [_p, _i, _i, _i, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p]),
+    'hcm_layer_norm_forward': (_i, [_p, _i, _i64, _i, _i64, _p, _i, _p, _i, _f, _p, _p, _p, _p, _i64, _p, _i64, _p]),
+    'hcm_layer_norm_backward_workspace_bytes': (_sz, [_i64, _i]),
+    'hcm_layer_norm_backward': (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i, _i64, _i, _p, _i, _p, _p, _p, _p, _p, _i, _p, _sz, _p]),
     'hcm_prof_enable': (_i, [_i]),
     'hcm_prof_read': (_i, [_p, _p]),
     'hcm_prof_read_tag': (_i, [_i, _p, _p]),

@@ -5,6 +5,7 @@ the C entry points of ``include/hcmoco_hip.h`` and wraps the result in a
 ``torch.autograd.Function`` where a backward exists.  No op has a CPU or eager fallback:
 CPU tensors raise ``RuntimeError`` and a missing library raises ``ImportError``.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -697,6 +698,175 @@ def bn_act(x, weight, bias, running_mean, running_var, momentum, eps, residual=N
     Runs as a C++ autograd node (csrc/torch_glue, torch.ops.hcmoco.bn_act) over hcm_bn_act_*."""
     return _lib.torch_glue().bn_act(x, residual, weight, bias, running_mean, running_var,
                                     float(momentum), float(eps), bool(relu))
+
+
+# --------------------------------------------------------------------------- #
+# 8-bit activation checkpoints (csrc/act8.hip) and layer norm (csrc/norm.hip)
+# --------------------------------------------------------------------------- #
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on(t):
+    """The device of ``t`` as the current one for the calls inside (streams and launches go by the current device)."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _float_dev(name, *ts):
+    """The tensors an operator reads are float32 / bfloat16 / float16, on one ROCm device."""
+    for t in ts:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError('hcmoco_amd.%s needs ROCm device tensors (no CPU fallback exists)' % name)
+        if t.dtype not in _DT:
+            raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, t.dtype))
+        if t.device != ts[0].device:
+            raise ValueError('%s: tensors on %s and on %s' % (name, ts[0].device, t.device))
+
+
+def _rows2d(x, name):
+    """x [..., C] as rows: (tensor that is read, rows, C, elements between rows).  A 2-D column slice is read where it lies."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError('%s: the last axis must have at least one element' % name)
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    if not x.is_contiguous():
+        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
+            return x, rows, cols, x.stride(0)
+        x = x.contiguous()
+    return x, rows, cols, cols
+
+
+def _ptr(t):
+    return C.c_void_p(0 if t is None else t.data_ptr())
+
+
+class Act8:
+    """A tensor held in 8 bits: ``q`` uint8 [rows, pitch] (e4m3 bytes) and ``scale`` uint8 [rows, blocks] (one power of two, as
+    exponent + 127, for 128 neighbouring values of a row; include/hcmoco_hip.h states the format), with the ``shape`` and
+    ``dtype`` of the tensor it stands for."""
+    __slots__ = ('q', 'scale', 'shape', 'dtype')
+
+    def __init__(self, q, scale, shape, dtype):
+        self.q, self.scale, self.shape, self.dtype = q, scale, torch.Size(shape), dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def nbytes(self):
+        return self.q.numel() + self.scale.numel()
+
+
+def _act8_buffers(rows, cols, device):
+    if cols > 2 ** 31 - 16385 or rows * ((cols + 127) // 128) >= 2 ** 31:
+        raise ValueError('act8: %d rows of %d values are too many (blocks of 128 are numbered in 31 bits)' % (rows, cols))
+    pitch, sp = (cols + 15) // 16 * 16, ((cols + 127) // 128 + 3) // 4 * 4
+    return (torch.empty(rows, pitch, dtype=torch.uint8, device=device), torch.empty(rows, sp, dtype=torch.uint8, device=device))
+
+
+@torch.no_grad()
+def act8_pack(x):
+    """``x`` [..., C] (float32 / bfloat16 / float16) -> :class:`Act8`: a byte a value and a byte for 128 of them.  The largest
+    relative error of a value within 2^14 of its block's largest is 2^-4 (half an e4m3 step); what lies further below is held to
+    2^-10 times the block's scale.  Values that are not finite read back as NaN, their neighbours are not disturbed."""
+    _float_dev('act8_pack', x)
+    xr, rows, cols, ldx = _rows2d(x, 'act8_pack')
+    q, scale = _act8_buffers(rows, cols, x.device)
+    if rows:
+        with _on(x):
+            check(_lib.lib().hcm_act8_pack(_ptr(xr), _DT[x.dtype], rows, cols, ldx, _ptr(q), q.shape[1], _ptr(scale), scale.shape[1],
+                                           _stream()), 'hcm_act8_pack')
+    return Act8(q, scale, x.shape, x.dtype)
+
+
+def _check_act8(p, name):
+    if not isinstance(p, Act8):
+        raise TypeError('%s: expected an Act8 (act8_pack), got %s' % (name, type(p).__name__))
+    cols = p.shape[-1]
+    rows = p.shape.numel() // cols
+    for t, width in ((p.q, (cols + 15) // 16 * 16), (p.scale, ((cols + 127) // 128 + 3) // 4 * 4)):
+        if not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous() or tuple(t.shape) != (rows, width) or t.device != p.q.device:
+            raise ValueError('%s: the buffers of the Act8 do not hold a tensor of shape %s' % (name, tuple(p.shape)))
+    if p.dtype not in _DT:
+        raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, p.dtype))
+    return rows, cols
+
+
+@torch.no_grad()
+def act8_unpack(p, dtype=None):
+    """The tensor an :class:`Act8` stands for, as ``dtype`` (its own by default), clamped to the type's largest finite value."""
+    rows, cols = _check_act8(p, 'act8_unpack')
+    dtype = p.dtype if dtype is None else dtype
+    if dtype not in _DT:
+        raise TypeError('act8_unpack: expected float32, bfloat16 or float16, got %s' % dtype)
+    x = torch.empty(p.shape, dtype=dtype, device=p.device)
+    if rows:
+        with _on(x):
+            check(_lib.lib().hcm_act8_unpack(_ptr(p.q), p.q.shape[1], _ptr(p.scale), p.scale.shape[1], rows, cols, _ptr(x), _DT[dtype],
+                                             _stream()), 'hcm_act8_unpack')
+    return x
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, act8):
+        xr, rows, cols, ldx = _rows2d(x, 'layer_norm')
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        need = any(ctx.needs_input_grad[:3])
+        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if need else None
+        q, scale = _act8_buffers(rows, cols, x.device) if need and act8 else (None, None)
+        if rows:
+            with _on(x):
+                check(_lib.lib().hcm_layer_norm_forward(
+                    _ptr(xr), _DT[x.dtype], rows, cols, ldx, _ptr(weight), _DT[weight.dtype] if weight is not None else 0, _ptr(bias),
+                    _DT[bias.dtype] if bias is not None else 0, eps, _ptr(y), C.c_void_p(stats.data_ptr() if need else 0),
+                    C.c_void_p(stats.data_ptr() + 4 * rows if need else 0), _ptr(q), 0 if q is None else q.shape[1], _ptr(scale),
+                    0 if q is None else scale.shape[1], _stream()), 'hcm_layer_norm_forward')
+        if need:
+            ctx.save_for_backward(*([q, scale] if act8 else [xr, None]), stats, weight)
+            ctx.dims = (rows, cols, ldx, act8, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        a, scale, stats, weight = ctx.saved_tensors
+        rows, cols, ldx, act8, bias_dtype = ctx.dims
+        dy = dy.contiguous()
+        dx = torch.empty_like(dy)
+        dw = torch.empty(cols, dtype=weight.dtype, device=dy.device) if ctx.needs_input_grad[1] else None
+        db = torch.empty(cols, dtype=bias_dtype, device=dy.device) if ctx.needs_input_grad[2] else None
+        if not rows:
+            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
+        L = _lib.lib()
+        nbytes = L.hcm_layer_norm_backward_workspace_bytes(rows, cols)
+        ws = _ws(nbytes, dy.device)
+        nul = C.c_void_p(0)
+        with _on(dy):
+            check(L.hcm_layer_norm_backward(
+                nul if act8 else _ptr(a), ldx, _ptr(a) if act8 else nul, a.shape[1] if act8 else 0, _ptr(scale), scale.shape[1] if act8 else 0,
+                _ptr(dy), _DT[dy.dtype], rows, cols, _ptr(weight), _DT[weight.dtype] if weight is not None else 0,
+                C.c_void_p(stats.data_ptr()), C.c_void_p(stats.data_ptr() + 4 * rows), _ptr(dx), _ptr(dw), _ptr(db),
+                _DT[bias_dtype] if db is not None else 0, _ptr(ws), nbytes, _stream()), 'hcm_layer_norm_backward')
+        return dx if ctx.needs_input_grad[0] else None, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, statistics in fp32, differentiable in x, weight and bias
+    (any may be float32 / bfloat16 / float16; a gradient has the type of what it belongs to).  ``act8``: the backward pass keeps x
+    as an 8-bit checkpoint (``act8_pack``'s format, written by the same kernel) instead of x itself, and computes its gradients
+    from the checkpoint's values with the exact mean and variance: a quarter of the memory for float32, at an error of up to
+    2^-4 of |x| in the normalised values that the gradients of weight and x are formed with.  Deterministic."""
+    _float_dev('layer_norm', x, weight, bias)
+    for p, what in ((weight, 'weight'), (bias, 'bias')):
+        if p is not None and (x.dim() == 0 or p.dim() != 1 or p.shape[0] != x.shape[-1] or not p.is_contiguous()):
+            raise ValueError('layer_norm: %s must be a contiguous vector as long as the last axis of x' % what)
+    if not eps >= 0:
+        raise ValueError('layer_norm: eps must not be negative')
+    return _LayerNorm.apply(x, weight, bias, float(eps), bool(act8))
 
 
 # --------------------------------------------------------------------------- #

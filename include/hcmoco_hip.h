@@ -718,6 +718,43 @@ int hcm_conv3x3_stats_slots(int N, int H);
 int hcm_conv3x3_forward_stats(const float* x, const float* w, float* y, int N, int C, int K, int H, int W, const float* shift,
                               float* partial_sums, hcm_stream_t stream);
 
+/* ------------------------------------------------------------------------ *
+ * 8-bit training operators: layer norm, 8-bit activation checkpoints, products of 8-bit blocks.
+ *
+ * Format.  128 neighbouring values of a row are held as e4m3 bytes q (OCP e4m3: +-448, one NaN, no infinity) times one power
+ * of two 2^E, E stored as the byte E + 127.  E is the smallest exponent with max|x| <= 448 * 2^E, at least -126, and 0 for a
+ * block of zeros; values that are not finite become NaN and do not count in the maximum.  q = round-to-nearest-even(x / 2^E).
+ *   q      [rows, ldq]  ldq = hcm_act8_pitch(cols): cols rounded up to 16, the pad is zero; 16-byte aligned
+ *   scale  [rows, lds]  lds = hcm_act8_scale_pitch(cols): ceil(cols / 128) rounded up to 4, the pad is 127
+ * A weight [rows, cols] has one E for each block of 128 x 128 and is held twice, as it lies and transposed.
+ * dtype codes: HCM_DT_*.  ldx: elements from one row of x to the next; any alignment.  rows * ceil(cols / 128) < 2^31.
+ * ------------------------------------------------------------------------ */
+#define HCM_DT_F32 0
+#define HCM_DT_BF16 1
+#define HCM_DT_F16 2
+int64_t hcm_act8_pitch(int64_t cols);
+int64_t hcm_act8_scale_pitch(int64_t cols);
+int hcm_act8_pack(const void* x, int dtype, int64_t rows, int cols, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                  hcm_stream_t stream);
+/* x [rows, cols] = q * 2^E, clamped to the type's largest finite value. */
+int hcm_act8_unpack(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int64_t rows, int cols, void* x, int dtype,
+                    hcm_stream_t stream);
+/* q [rows, ldq], scale [ceil(rows / 128), lds]; qt [cols, ldqt], scale_t [ceil(cols / 128), ldst] with the pitches of `rows`. */
+int hcm_fp8_weight_pack(const void* w, int dtype, int rows, int cols, int64_t ldw, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                        uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, hcm_stream_t stream);
+
+/* Layer norm over the last axis: y [rows, cols] = (x - mean) / sqrt(var + eps) * w + b; sums in fp32.  w, b: NULL = 1, 0.
+ * mean, rstd [rows] fp32: NULL when no backward pass follows.  q, scale: NULL, or the 8-bit checkpoint of x is written too.
+ * Backward takes either x or its checkpoint (the other NULL); dw, db: NULL = not wanted; fixed order, no atomics. */
+int hcm_layer_norm_forward(const void* x, int dtype, int64_t rows, int cols, int64_t ldx, const void* w, int w_dtype, const void* b,
+                           int b_dtype, float eps, void* y, float* mean, float* rstd, uint8_t* q, int64_t ldq, uint8_t* scale,
+                           int64_t lds, hcm_stream_t stream);
+size_t hcm_layer_norm_backward_workspace_bytes(int64_t rows, int cols);
+int hcm_layer_norm_backward(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds,
+                            const void* dy, int dtype, int64_t rows, int cols, const void* w, int w_dtype, const float* mean,
+                            const float* rstd, void* dx, void* dw, void* db, int b_dtype, void* workspace, size_t workspace_bytes,
+                            hcm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

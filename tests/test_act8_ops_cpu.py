@@ -1,0 +1,71 @@
+"""What the 8-bit training operators refuse without a GPU: CPU tensors, and at the C ABI every size, pitch and pointer that a kernel
+does not take (all checked before anything is launched)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from act8_ref import held8
+from hcmoco_amd import _lib, hip_ops
+
+Z, P = C.c_void_p(0), C.c_void_p(4096)      # P: never read, the call ends at its checks
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.zeros(8)
+    for call in (lambda: hip_ops.act8_pack(x), lambda: hip_ops.layer_norm(x), lambda: hip_ops.layer_norm(x, w, w, act8=True)):
+        with pytest.raises(RuntimeError, match='no CPU fallback'):
+            call()
+
+
+def test_pitches():
+    L = _lib.lib()
+    for c, p, s in ((1, 16, 4), (16, 16, 4), (17, 32, 4), (128, 128, 4), (512, 512, 4), (513, 528, 8), (1290, 1296, 12)):
+        assert (L.hcm_act8_pitch(c), L.hcm_act8_scale_pitch(c)) == (p, s)
+
+
+def test_pack_refuses():
+    L = _lib.lib()
+    good = dict(x=P, dt=0, rows=4, cols=270, ldx=270, q=P, ldq=272, s=P, lds=4)
+    for bad in (dict(x=Z), dict(dt=3), dict(dt=-1), dict(rows=0), dict(rows=-1), dict(cols=0), dict(ldx=269), dict(q=Z), dict(q=C.c_void_p(4100)),
+                dict(ldq=270), dict(ldq=288), dict(s=Z), dict(lds=3), dict(rows=2 ** 31)):
+        a = {**good, **bad}
+        assert L.hcm_act8_pack(a['x'], a['dt'], a['rows'], a['cols'], a['ldx'], a['q'], a['ldq'], a['s'], a['lds'], Z) != 0, bad
+        if 'ldx' not in bad:
+            assert L.hcm_act8_unpack(a['q'], a['ldq'], a['s'], a['lds'], a['rows'], a['cols'], a['x'], a['dt'], Z) != 0, bad
+
+
+def test_weight_pack_refuses():
+    L = _lib.lib()
+    good = dict(w=P, dt=0, rows=200, cols=270, ldw=270, q=P, ldq=272, s=P, lds=4, qt=P, ldqt=208, st=P, ldst=4)
+    for bad in (dict(w=Z), dict(dt=7), dict(rows=0), dict(cols=0), dict(ldw=1), dict(q=Z), dict(ldq=270), dict(s=Z), dict(lds=8), dict(qt=Z),
+                dict(ldqt=200), dict(st=Z), dict(ldst=2), dict(qt=C.c_void_p(4104))):
+        a = {**good, **bad}
+        assert L.hcm_fp8_weight_pack(*[a[k] for k in good], Z) != 0, bad
+
+
+def test_layer_norm_refuses():
+    L = _lib.lib()
+    good = dict(x=P, dt=0, rows=4, cols=270, ldx=270, w=Z, wd=0, b=Z, bd=0, eps=1e-5, y=P, mean=P, rstd=P, q=P, ldq=272, s=P, lds=4)
+    for bad in (dict(x=Z), dict(dt=3), dict(rows=0), dict(rows=2 ** 31), dict(cols=0), dict(ldx=269), dict(wd=5), dict(bd=-2), dict(y=Z), dict(mean=Z),
+                dict(s=Z), dict(q=C.c_void_p(4100)), dict(ldq=270), dict(lds=1)):
+        a = {**good, **bad}
+        assert L.hcm_layer_norm_forward(*[a[k] for k in good], Z) != 0, bad
+    need = L.hcm_layer_norm_backward_workspace_bytes(4, 270)
+    assert need > 0 and L.hcm_layer_norm_backward_workspace_bytes(0, 270) == 0
+    good = dict(x=P, ldx=270, q=Z, ldq=0, s=Z, lds=0, dy=P, dt=0, rows=4, cols=270, w=Z, wd=0, mean=P, rstd=P, dx=P, dw=P, db=P, bd=0, ws=P, n=need)
+    for bad in (dict(x=Z), dict(q=P), dict(q=P, s=P), dict(x=Z, q=P, s=P, ldq=270, lds=4), dict(dy=Z), dict(rows=0), dict(dx=Z), dict(mean=Z),
+                dict(ws=Z), dict(n=need - 1), dict(dt=4), dict(ldx=3)):
+        a = {**good, **bad}
+        assert L.hcm_layer_norm_backward(*[a[k] for k in good], Z) != 0, bad
+
+
+def test_the_format_of_the_reference_matches_torchs_e4m3():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 300, generator=g) * torch.exp(4 * torch.randn(50, 1, generator=g))
+    val, e = held8(x)
+    s = torch.repeat_interleave(torch.exp2(e.double()), 128, 1)[:, :300]
+    assert torch.equal((x.double() / s).float().to(torch.float8_e4m3fn).double() * s, val)
+    assert (x.double() / s).abs().max() <= 448
+    blocks = torch.nn.functional.pad((x.double() / s).abs(), (0, 84)).view(50, 3, 128).amax(2)
+    assert (blocks > 224).all()                            # a smaller power of two would not have held the block
