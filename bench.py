@@ -329,6 +329,17 @@ class FailSafe(object):
                 except OSError:
                     sigs = []
                 if sigs:
+                    # a peer that left a note and ended makes the launcher send this signal: the note, written before the peer
+                    # ended, may not have been seen by the poll below yet
+                    try:
+                        with self.store_lock:
+                            hit = [k for k in ('hcm_bench_error/%d' % r_ for r_ in range(1, self.world)) if self.store.check([k])]
+                            note = self.store.get(hit[0]).decode(errors='replace') if hit else None
+                        if hit:
+                            self.emit('%s: %s || rank 0 then received signal %s' % (hit[0], note, sigs))
+                            os._exit(3)
+                    except Exception:         # noqa: BLE001 -- no store, or gone: the signal is all there is
+                        pass
                     self.emit('rank 0 received signal %s in phase %r: the launcher tore the job down (a peer rank died?)'
                               % (sigs, self.phase))
                     os._exit(3)
