@@ -870,6 +870,147 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
 
 
 # --------------------------------------------------------------------------- #
+# linear layers on 8-bit blocks (csrc/fp8mm.hip)
+# --------------------------------------------------------------------------- #
+class Fp8Weight:
+    """A weight [N, K] held in 8 bits: e4m3 bytes with one power of two for each block of 128 x 128, as it lies (``q``, ``scale``)
+    and transposed (``qt``, ``scale_t``: what the gradient of the input is multiplied with).  Made by :func:`fp8_weight`."""
+    __slots__ = ('q', 'scale', 'qt', 'scale_t', 'shape', 'dtype')
+
+    def __init__(self, q, scale, qt, scale_t, shape, dtype):
+        self.q, self.scale, self.qt, self.scale_t, self.shape, self.dtype = q, scale, qt, scale_t, torch.Size(shape), dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    def nbytes(self):
+        return self.q.numel() + self.scale.numel() + self.qt.numel() + self.scale_t.numel()
+
+
+_FP8_MAX = 1 << 22      # the largest N and K of a product
+
+
+@torch.no_grad()
+def fp8_weight(weight):
+    """``weight`` [N, K] (float32 / bfloat16 / float16) -> :class:`Fp8Weight`, laid out once for any number of products."""
+    _float_dev('fp8_weight', weight)
+    if weight.dim() != 2 or not (0 < weight.shape[0] <= _FP8_MAX and 0 < weight.shape[1] <= _FP8_MAX):
+        raise ValueError('fp8_weight: expected [N, K] with both in 1..2^22, got %s' % (tuple(weight.shape),))
+    w, N, K, ldw = _rows2d(weight, 'fp8_weight')
+    q, qt = _act8_buffers(N, K, w.device)[0], _act8_buffers(K, N, w.device)[0]
+    scale = torch.empty((N + 127) // 128, ((K + 127) // 128 + 3) // 4 * 4, dtype=torch.uint8, device=w.device)
+    scale_t = torch.empty((K + 127) // 128, ((N + 127) // 128 + 3) // 4 * 4, dtype=torch.uint8, device=w.device)
+    with _on(w):
+        check(_lib.lib().hcm_fp8_weight_pack(_ptr(w), _DT[w.dtype], N, K, ldw, _ptr(q), q.shape[1], _ptr(scale), scale.shape[1], _ptr(qt),
+                                             qt.shape[1], _ptr(scale_t), scale_t.shape[1], _stream()), 'hcm_fp8_weight_pack')
+    return Fp8Weight(q, scale, qt, scale_t, weight.shape, weight.dtype)
+
+
+def _fp8_product(xq, xs, M, wq, ws, N, K, bias, dtype):
+    """[M, N] = X W^T + bias on packed buffers whose sizes the caller has checked."""
+    y = torch.empty(M, N, dtype=dtype, device=xq.device)
+    if M:
+        L = _lib.lib()
+        nbytes = L.hcm_fp8_matmul_workspace_bytes(M, N, K, _DT[dtype])
+        work = _ws(nbytes, xq.device) if nbytes else None
+        with _on(xq):
+            check(L.hcm_fp8_matmul(_ptr(xq), xq.shape[1], _ptr(xs), xs.shape[1], _ptr(wq), wq.shape[1], _ptr(ws), ws.shape[1], _ptr(bias),
+                                   _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(y), _DT[dtype], _ptr(work), nbytes,
+                                   _stream()), 'hcm_fp8_matmul')
+    return y
+
+
+def _fp8_wgrad(xq, xs, dy, M, N, K, dw, db):
+    L = _lib.lib()
+    nbytes = L.hcm_fp8_wgrad_workspace_bytes(M, N, K)
+    work = _ws(nbytes, dy.device)
+    with _on(dy):
+        check(L.hcm_fp8_wgrad(_ptr(xq), xq.shape[1], _ptr(xs), xs.shape[1], _ptr(dy), _DT[dy.dtype], M, N, K, _ptr(dw),
+                              _DT[dw.dtype] if dw is not None else 0, _ptr(db), _DT[db.dtype] if db is not None else 0, _ptr(work), nbytes,
+                              _stream()), 'hcm_fp8_wgrad')
+
+
+def _check_fp8(x_cols, x_device, w, bias, name):
+    if len(w.shape) != 2 or w.shape[1] != x_cols:
+        raise ValueError('%s: a weight of shape %s does not go with %d values a row' % (name, tuple(w.shape), x_cols))
+    if w.device != x_device:
+        raise ValueError('%s: tensors on %s and on %s' % (name, x_device, w.device))
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != w.shape[0] or not bias.is_contiguous()):
+        raise ValueError('%s: bias must be a contiguous vector of %d values' % (name, w.shape[0]))
+
+
+@torch.no_grad()
+def fp8_matmul(a, weight, bias=None, dtype=None):
+    """``a`` (:class:`Act8`, [..., K]) times ``weight`` (:class:`Fp8Weight`, [N, K]) transposed, plus ``bias``: [..., N] as ``dtype`` (the
+    type ``a`` stands for by default).  8-bit products, fp32 sums.  Not differentiable: :func:`fp8_linear` is."""
+    rows, cols = _check_act8(a, 'fp8_matmul')
+    if not isinstance(weight, Fp8Weight):
+        raise TypeError('fp8_matmul: expected an Fp8Weight (fp8_weight), got %s' % type(weight).__name__)
+    _float_dev('fp8_matmul', *([bias] if bias is not None else []))
+    _check_fp8(cols, a.device, weight, bias, 'fp8_matmul')
+    if bias is not None and bias.device != a.device:
+        raise ValueError('fp8_matmul: tensors on %s and on %s' % (a.device, bias.device))
+    dtype = a.dtype if dtype is None else dtype
+    if dtype not in _DT:
+        raise TypeError('fp8_matmul: expected float32, bfloat16 or float16, got %s' % dtype)
+    y = _fp8_product(a.q, a.scale, rows, weight.q, weight.scale, weight.shape[0], cols, bias, dtype)
+    return y.view(a.shape[:-1] + (weight.shape[0],))
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, packed):
+        w = fp8_weight(weight) if packed is None else packed
+        a = act8_pack(x)
+        N, K = w.shape
+        rows = a.q.shape[0]
+        y = _fp8_product(a.q, a.scale, rows, w.q, w.scale, N, K, bias, x.dtype)
+        if any(ctx.needs_input_grad[:3]):
+            # x itself is not kept: the 8-bit operand of this product is the checkpoint that the weight gradient reads
+            ctx.save_for_backward(a.q, a.scale, w.qt, w.scale_t)
+            ctx.dims = (rows, N, K, x.shape, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y.view(x.shape[:-1] + (N,))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, scale, qt, scale_t = ctx.saved_tensors
+        rows, N, K, x_shape, w_dtype, b_dtype = ctx.dims
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev, dtype = dy.device, dy.dtype
+        dx = None
+        dw = torch.empty(N, K, dtype=w_dtype, device=dev) if need_w else None
+        db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
+        if not rows:
+            return (torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None, None if dw is None else dw.zero_(),
+                    None if db is None else db.zero_(), None)
+        dy = dy.reshape(rows, N).contiguous()
+        if need_x:
+            g = act8_pack(dy)
+            dx = _fp8_product(g.q, g.scale, rows, qt, scale_t, K, N, None, dtype).view(x_shape)
+        if need_w or need_b:
+            _fp8_wgrad(q, scale, dy, rows, N, K, dw, db)
+        return dx, dw, db, None
+
+
+def fp8_linear(x, weight, bias=None):
+    """x [..., K] times weight [N, K] transposed, plus bias, on 8-bit blocks: y = Q(x) Q(weight)^T + bias, in x's type, fp32 sums.
+
+    ``weight``: a tensor, which is laid out anew on every call (training), or an :class:`Fp8Weight` that the caller keeps
+    (inference, or a frozen layer).  Differentiable in x, bias and a weight tensor; Q counts as the identity there:
+    dx = Q(dy) Q(weight), dweight = dy^T Q(x), dbias = sum of dy.  The backward pass keeps Q(x), a byte a value, and not x; dy enters
+    the weight's gradient unrounded.  Q is the format of :func:`act8_pack`: rows of x and dy in blocks of 128, the weight in blocks
+    of 128 x 128.  Deterministic."""
+    packed = weight if isinstance(weight, Fp8Weight) else None
+    _float_dev('fp8_linear', x, *([weight] if packed is None else []), *([bias] if bias is not None else []))
+    if x.dim() == 0:
+        raise ValueError('fp8_linear: x needs at least one axis')
+    _check_fp8(x.shape[-1], x.device, weight, bias, 'fp8_linear')
+    return _Fp8Linear.apply(x, None if packed is not None else weight, bias, packed)
+
+
+# --------------------------------------------------------------------------- #
 # weight gradient of the 3x3 / stride 1 / pad 1 encoder convolutions
 # --------------------------------------------------------------------------- #
 def conv3x3_wgrad(x, dy, ksize=3, stride=1):

@@ -13,7 +13,8 @@ Z, P = C.c_void_p(0), C.c_void_p(4096)      # P: never read, the call ends at it
 
 def test_cpu_tensors_are_refused():
     x, w = torch.zeros(4, 8), torch.zeros(8)
-    for call in (lambda: hip_ops.act8_pack(x), lambda: hip_ops.layer_norm(x), lambda: hip_ops.layer_norm(x, w, w, act8=True)):
+    for call in (lambda: hip_ops.act8_pack(x), lambda: hip_ops.layer_norm(x), lambda: hip_ops.layer_norm(x, w, w, act8=True),
+                 lambda: hip_ops.fp8_weight(x), lambda: hip_ops.fp8_linear(x, x)):
         with pytest.raises(RuntimeError, match='no CPU fallback'):
             call()
 
@@ -58,6 +59,27 @@ def test_layer_norm_refuses():
                 dict(ws=Z), dict(n=need - 1), dict(dt=4), dict(ldx=3)):
         a = {**good, **bad}
         assert L.hcm_layer_norm_backward(*[a[k] for k in good], Z) != 0, bad
+
+
+def test_products_refuse():
+    L = _lib.lib()
+    good = dict(x=P, ldx=272, sx=P, ldsx=4, w=P, ldw=272, sw=P, ldsw=4, b=Z, bd=0, M=4, N=200, K=270, y=P, od=0, ws=P, n=1 << 30)
+    for bad in (dict(x=Z), dict(ldx=270), dict(sx=Z), dict(ldsx=3), dict(w=Z), dict(ldw=288), dict(sw=Z), dict(ldsw=8), dict(b=P, bd=3), dict(M=0),
+                dict(M=2 ** 31 - 1), dict(N=0), dict(N=2 ** 22 + 1), dict(K=0), dict(K=2 ** 22 + 1), dict(y=Z), dict(od=-1), dict(od=3),
+                dict(x=C.c_void_p(4104)), dict(w=C.c_void_p(4104))):
+        a = {**good, **bad}
+        assert L.hcm_fp8_matmul(*[a[k] for k in good], Z) != 0, bad
+    need = L.hcm_fp8_matmul_workspace_bytes(32, 128, 4096, 0)
+    assert need > 0 and L.hcm_fp8_matmul_workspace_bytes(8192, 8192, 8192, 1) == 0 and L.hcm_fp8_matmul_workspace_bytes(0, 1, 1, 0) == 0
+    a = {**good, **dict(ldx=4096, ldw=4096, ldsx=32, ldsw=32, M=32, N=128, K=4096)}
+    for bad in (dict(n=need - 1), dict(ws=Z)):
+        assert L.hcm_fp8_matmul(*[{**a, **bad}[k] for k in good], Z) != 0, bad
+    need = L.hcm_fp8_wgrad_workspace_bytes(1000, 200, 270)
+    good = dict(x=P, ldx=272, sx=P, ldsx=4, dy=P, dd=0, M=1000, N=200, K=270, dw=P, wd=0, db=P, bd=0, ws=P, n=need)
+    for bad in (dict(x=Z), dict(ldx=270), dict(sx=Z), dict(ldsx=2), dict(dy=Z), dict(dd=3), dict(M=0), dict(M=2 ** 31), dict(N=0), dict(K=0),
+                dict(N=2 ** 22 + 1), dict(dw=Z, db=Z), dict(wd=9), dict(bd=-1), dict(ws=Z), dict(n=need - 1), dict(x=C.c_void_p(4104))):
+        a = {**good, **bad}
+        assert L.hcm_fp8_wgrad(*[a[k] for k in good], Z) != 0, bad
 
 
 def test_the_format_of_the_reference_matches_torchs_e4m3():
