@@ -5,7 +5,6 @@ the C entry points of ``include/hcmoco_hip.h`` and wraps the result in a
 ``torch.autograd.Function`` where a backward exists.  No op has a CPU or eager fallback:
 CPU tensors raise ``RuntimeError`` and a missing library raises ``ImportError``.
 """
-import contextlib
 import ctypes as C
 import os
 
@@ -701,52 +700,14 @@ def bn_act(x, weight, bias, running_mean, running_var, momentum, eps, residual=N
 
 
 # --------------------------------------------------------------------------- #
-# 8-bit activation checkpoints (csrc/act8.hip) and layer norm (csrc/norm.hip)
+# 8-bit activation checkpoints (csrc/act8.hip), layer norm (csrc/norm.hip), linear layers on 8-bit blocks (csrc/fp8mm.hip).
+# The autograd nodes and every check of arguments are C++ (csrc/torch_glue/act8_glue.cpp): TypeError for a type, ValueError
+# for a shape or a mixture of devices, RuntimeError for CPU tensors.
 # --------------------------------------------------------------------------- #
-_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _on(t):
-    """The device of ``t`` as the current one for the calls inside (streams and launches go by the current device)."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-def _float_dev(name, *ts):
-    """The tensors an operator reads are float32 / bfloat16 / float16, on one ROCm device."""
-    for t in ts:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise RuntimeError('hcmoco_amd.%s needs ROCm device tensors (no CPU fallback exists)' % name)
-        if t.dtype not in _DT:
-            raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, t.dtype))
-        if t.device != ts[0].device:
-            raise ValueError('%s: tensors on %s and on %s' % (name, ts[0].device, t.device))
-
-
-def _rows2d(x, name):
-    """x [..., C] as rows: (tensor that is read, rows, C, elements between rows).  A 2-D column slice is read where it lies."""
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError('%s: the last axis must have at least one element' % name)
-    cols = x.shape[-1]
-    rows = x.numel() // cols
-    if not x.is_contiguous():
-        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= cols:
-            return x, rows, cols, x.stride(0)
-        x = x.contiguous()
-    return x, rows, cols, cols
-
-
-def _ptr(t):
-    return C.c_void_p(0 if t is None else t.data_ptr())
-
-
 class Act8:
     """A tensor held in 8 bits: ``q`` uint8 [rows, pitch] (e4m3 bytes) and ``scale`` uint8 [rows, blocks] (one power of two, as
     exponent + 127, for 128 neighbouring values of a row; include/hcmoco_hip.h states the format), with the ``shape`` and
-    ``dtype`` of the tensor it stands for."""
+    ``dtype`` of the tensor it stands for.  Made by :func:`act8_pack`."""
     __slots__ = ('q', 'scale', 'shape', 'dtype')
 
     def __init__(self, q, scale, shape, dtype):
@@ -760,98 +721,22 @@ class Act8:
         return self.q.numel() + self.scale.numel()
 
 
-def _act8_buffers(rows, cols, device):
-    if cols > 2 ** 31 - 16385 or rows * ((cols + 127) // 128) >= 2 ** 31:
-        raise ValueError('act8: %d rows of %d values are too many (blocks of 128 are numbered in 31 bits)' % (rows, cols))
-    pitch, sp = (cols + 15) // 16 * 16, ((cols + 127) // 128 + 3) // 4 * 4
-    return (torch.empty(rows, pitch, dtype=torch.uint8, device=device), torch.empty(rows, sp, dtype=torch.uint8, device=device))
-
-
 @torch.no_grad()
 def act8_pack(x):
     """``x`` [..., C] (float32 / bfloat16 / float16) -> :class:`Act8`: a byte a value and a byte for 128 of them.  The largest
     relative error of a value within 2^14 of its block's largest is 2^-4 (half an e4m3 step); what lies further below is held to
-    2^-10 times the block's scale.  Values that are not finite read back as NaN, their neighbours are not disturbed."""
-    _float_dev('act8_pack', x)
-    xr, rows, cols, ldx = _rows2d(x, 'act8_pack')
-    q, scale = _act8_buffers(rows, cols, x.device)
-    if rows:
-        with _on(x):
-            check(_lib.lib().hcm_act8_pack(_ptr(xr), _DT[x.dtype], rows, cols, ldx, _ptr(q), q.shape[1], _ptr(scale), scale.shape[1],
-                                           _stream()), 'hcm_act8_pack')
+    2^-10 times the block's scale.  Values that are not finite read back as NaN, their neighbours are not disturbed.  Rows may
+    be a column slice of a wider matrix; any other view is copied first."""
+    q, scale = _lib.torch_glue().act8_pack(x)
     return Act8(q, scale, x.shape, x.dtype)
-
-
-def _check_act8(p, name):
-    if not isinstance(p, Act8):
-        raise TypeError('%s: expected an Act8 (act8_pack), got %s' % (name, type(p).__name__))
-    cols = p.shape[-1]
-    rows = p.shape.numel() // cols
-    for t, width in ((p.q, (cols + 15) // 16 * 16), (p.scale, ((cols + 127) // 128 + 3) // 4 * 4)):
-        if not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous() or tuple(t.shape) != (rows, width) or t.device != p.q.device:
-            raise ValueError('%s: the buffers of the Act8 do not hold a tensor of shape %s' % (name, tuple(p.shape)))
-    if p.dtype not in _DT:
-        raise TypeError('%s: expected float32, bfloat16 or float16, got %s' % (name, p.dtype))
-    return rows, cols
 
 
 @torch.no_grad()
 def act8_unpack(p, dtype=None):
     """The tensor an :class:`Act8` stands for, as ``dtype`` (its own by default), clamped to the type's largest finite value."""
-    rows, cols = _check_act8(p, 'act8_unpack')
-    dtype = p.dtype if dtype is None else dtype
-    if dtype not in _DT:
-        raise TypeError('act8_unpack: expected float32, bfloat16 or float16, got %s' % dtype)
-    x = torch.empty(p.shape, dtype=dtype, device=p.device)
-    if rows:
-        with _on(x):
-            check(_lib.lib().hcm_act8_unpack(_ptr(p.q), p.q.shape[1], _ptr(p.scale), p.scale.shape[1], rows, cols, _ptr(x), _DT[dtype],
-                                             _stream()), 'hcm_act8_unpack')
-    return x
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, act8):
-        xr, rows, cols, ldx = _rows2d(x, 'layer_norm')
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        need = any(ctx.needs_input_grad[:3])
-        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if need else None
-        q, scale = _act8_buffers(rows, cols, x.device) if need and act8 else (None, None)
-        if rows:
-            with _on(x):
-                check(_lib.lib().hcm_layer_norm_forward(
-                    _ptr(xr), _DT[x.dtype], rows, cols, ldx, _ptr(weight), _DT[weight.dtype] if weight is not None else 0, _ptr(bias),
-                    _DT[bias.dtype] if bias is not None else 0, eps, _ptr(y), C.c_void_p(stats.data_ptr() if need else 0),
-                    C.c_void_p(stats.data_ptr() + 4 * rows if need else 0), _ptr(q), 0 if q is None else q.shape[1], _ptr(scale),
-                    0 if q is None else scale.shape[1], _stream()), 'hcm_layer_norm_forward')
-        if need:
-            ctx.save_for_backward(*([q, scale] if act8 else [xr, None]), stats, weight)
-            ctx.dims = (rows, cols, ldx, act8, None if bias is None else bias.dtype)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        a, scale, stats, weight = ctx.saved_tensors
-        rows, cols, ldx, act8, bias_dtype = ctx.dims
-        dy = dy.contiguous()
-        dx = torch.empty_like(dy)
-        dw = torch.empty(cols, dtype=weight.dtype, device=dy.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(cols, dtype=bias_dtype, device=dy.device) if ctx.needs_input_grad[2] else None
-        if not rows:
-            return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
-        L = _lib.lib()
-        nbytes = L.hcm_layer_norm_backward_workspace_bytes(rows, cols)
-        ws = _ws(nbytes, dy.device)
-        nul = C.c_void_p(0)
-        with _on(dy):
-            check(L.hcm_layer_norm_backward(
-                nul if act8 else _ptr(a), ldx, _ptr(a) if act8 else nul, a.shape[1] if act8 else 0, _ptr(scale), scale.shape[1] if act8 else 0,
-                _ptr(dy), _DT[dy.dtype], rows, cols, _ptr(weight), _DT[weight.dtype] if weight is not None else 0,
-                C.c_void_p(stats.data_ptr()), C.c_void_p(stats.data_ptr() + 4 * rows), _ptr(dx), _ptr(dw), _ptr(db),
-                _DT[bias_dtype] if db is not None else 0, _ptr(ws), nbytes, _stream()), 'hcm_layer_norm_backward')
-        return dx if ctx.needs_input_grad[0] else None, dw, db, None, None
+    if not isinstance(p, Act8):
+        raise TypeError('act8_unpack: expected an Act8 (act8_pack), got %s' % type(p).__name__)
+    return _lib.torch_glue().act8_unpack(p.q, p.scale, p.shape, p.dtype if dtype is None else dtype)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
@@ -859,19 +744,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
     (any may be float32 / bfloat16 / float16; a gradient has the type of what it belongs to).  ``act8``: the backward pass keeps x
     as an 8-bit checkpoint (``act8_pack``'s format, written by the same kernel) instead of x itself, and computes its gradients
     from the checkpoint's values with the exact mean and variance: a quarter of the memory for float32, at an error of up to
-    2^-4 of |x| in the normalised values that the gradients of weight and x are formed with.  Deterministic."""
-    _float_dev('layer_norm', x, weight, bias)
-    for p, what in ((weight, 'weight'), (bias, 'bias')):
-        if p is not None and (x.dim() == 0 or p.dim() != 1 or p.shape[0] != x.shape[-1] or not p.is_contiguous()):
-            raise ValueError('layer_norm: %s must be a contiguous vector as long as the last axis of x' % what)
-    if not eps >= 0:
-        raise ValueError('layer_norm: eps must not be negative')
-    return _LayerNorm.apply(x, weight, bias, float(eps), bool(act8))
+    2^-4 of |x| in the normalised values that the gradients of weight and x are formed with.  Deterministic; no second
+    derivative."""
+    return _lib.torch_glue().layer_norm(x, weight, bias, float(eps), bool(act8))
 
 
-# --------------------------------------------------------------------------- #
-# linear layers on 8-bit blocks (csrc/fp8mm.hip)
-# --------------------------------------------------------------------------- #
 class Fp8Weight:
     """A weight [N, K] held in 8 bits: e4m3 bytes with one power of two for each block of 128 x 128, as it lies (``q``, ``scale``)
     and transposed (``qt``, ``scale_t``: what the gradient of the input is multiplied with).  Made by :func:`fp8_weight`."""
@@ -888,126 +765,34 @@ class Fp8Weight:
         return self.q.numel() + self.scale.numel() + self.qt.numel() + self.scale_t.numel()
 
 
-_FP8_MAX = 1 << 22      # the largest N and K of a product
-
-
 @torch.no_grad()
 def fp8_weight(weight):
     """``weight`` [N, K] (float32 / bfloat16 / float16) -> :class:`Fp8Weight`, laid out once for any number of products."""
-    _float_dev('fp8_weight', weight)
-    if weight.dim() != 2 or not (0 < weight.shape[0] <= _FP8_MAX and 0 < weight.shape[1] <= _FP8_MAX):
-        raise ValueError('fp8_weight: expected [N, K] with both in 1..2^22, got %s' % (tuple(weight.shape),))
-    w, N, K, ldw = _rows2d(weight, 'fp8_weight')
-    q, qt = _act8_buffers(N, K, w.device)[0], _act8_buffers(K, N, w.device)[0]
-    scale = torch.empty((N + 127) // 128, ((K + 127) // 128 + 3) // 4 * 4, dtype=torch.uint8, device=w.device)
-    scale_t = torch.empty((K + 127) // 128, ((N + 127) // 128 + 3) // 4 * 4, dtype=torch.uint8, device=w.device)
-    with _on(w):
-        check(_lib.lib().hcm_fp8_weight_pack(_ptr(w), _DT[w.dtype], N, K, ldw, _ptr(q), q.shape[1], _ptr(scale), scale.shape[1], _ptr(qt),
-                                             qt.shape[1], _ptr(scale_t), scale_t.shape[1], _stream()), 'hcm_fp8_weight_pack')
-    return Fp8Weight(q, scale, qt, scale_t, weight.shape, weight.dtype)
-
-
-def _fp8_product(xq, xs, M, wq, ws, N, K, bias, dtype):
-    """[M, N] = X W^T + bias on packed buffers whose sizes the caller has checked."""
-    y = torch.empty(M, N, dtype=dtype, device=xq.device)
-    if M:
-        L = _lib.lib()
-        nbytes = L.hcm_fp8_matmul_workspace_bytes(M, N, K, _DT[dtype])
-        work = _ws(nbytes, xq.device) if nbytes else None
-        with _on(xq):
-            check(L.hcm_fp8_matmul(_ptr(xq), xq.shape[1], _ptr(xs), xs.shape[1], _ptr(wq), wq.shape[1], _ptr(ws), ws.shape[1], _ptr(bias),
-                                   _DT[bias.dtype] if bias is not None else 0, M, N, K, _ptr(y), _DT[dtype], _ptr(work), nbytes,
-                                   _stream()), 'hcm_fp8_matmul')
-    return y
-
-
-def _fp8_wgrad(xq, xs, dy, M, N, K, dw, db):
-    L = _lib.lib()
-    nbytes = L.hcm_fp8_wgrad_workspace_bytes(M, N, K)
-    work = _ws(nbytes, dy.device)
-    with _on(dy):
-        check(L.hcm_fp8_wgrad(_ptr(xq), xq.shape[1], _ptr(xs), xs.shape[1], _ptr(dy), _DT[dy.dtype], M, N, K, _ptr(dw),
-                              _DT[dw.dtype] if dw is not None else 0, _ptr(db), _DT[db.dtype] if db is not None else 0, _ptr(work), nbytes,
-                              _stream()), 'hcm_fp8_wgrad')
-
-
-def _check_fp8(x_cols, x_device, w, bias, name):
-    if len(w.shape) != 2 or w.shape[1] != x_cols:
-        raise ValueError('%s: a weight of shape %s does not go with %d values a row' % (name, tuple(w.shape), x_cols))
-    if w.device != x_device:
-        raise ValueError('%s: tensors on %s and on %s' % (name, x_device, w.device))
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != w.shape[0] or not bias.is_contiguous()):
-        raise ValueError('%s: bias must be a contiguous vector of %d values' % (name, w.shape[0]))
+    return Fp8Weight(*_lib.torch_glue().fp8_weight(weight), weight.shape, weight.dtype)
 
 
 @torch.no_grad()
 def fp8_matmul(a, weight, bias=None, dtype=None):
     """``a`` (:class:`Act8`, [..., K]) times ``weight`` (:class:`Fp8Weight`, [N, K]) transposed, plus ``bias``: [..., N] as ``dtype`` (the
-    type ``a`` stands for by default).  8-bit products, fp32 sums.  Not differentiable: :func:`fp8_linear` is."""
-    rows, cols = _check_act8(a, 'fp8_matmul')
-    if not isinstance(weight, Fp8Weight):
-        raise TypeError('fp8_matmul: expected an Fp8Weight (fp8_weight), got %s' % type(weight).__name__)
-    _float_dev('fp8_matmul', *([bias] if bias is not None else []))
-    _check_fp8(cols, a.device, weight, bias, 'fp8_matmul')
-    if bias is not None and bias.device != a.device:
-        raise ValueError('fp8_matmul: tensors on %s and on %s' % (a.device, bias.device))
-    dtype = a.dtype if dtype is None else dtype
-    if dtype not in _DT:
-        raise TypeError('fp8_matmul: expected float32, bfloat16 or float16, got %s' % dtype)
-    y = _fp8_product(a.q, a.scale, rows, weight.q, weight.scale, weight.shape[0], cols, bias, dtype)
-    return y.view(a.shape[:-1] + (weight.shape[0],))
-
-
-class _Fp8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, packed):
-        w = fp8_weight(weight) if packed is None else packed
-        a = act8_pack(x)
-        N, K = w.shape
-        rows = a.q.shape[0]
-        y = _fp8_product(a.q, a.scale, rows, w.q, w.scale, N, K, bias, x.dtype)
-        if any(ctx.needs_input_grad[:3]):
-            # x itself is not kept: the 8-bit operand of this product is the checkpoint that the weight gradient reads
-            ctx.save_for_backward(a.q, a.scale, w.qt, w.scale_t)
-            ctx.dims = (rows, N, K, x.shape, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y.view(x.shape[:-1] + (N,))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        q, scale, qt, scale_t = ctx.saved_tensors
-        rows, N, K, x_shape, w_dtype, b_dtype = ctx.dims
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev, dtype = dy.device, dy.dtype
-        dx = None
-        dw = torch.empty(N, K, dtype=w_dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=b_dtype, device=dev) if need_b else None
-        if not rows:
-            return (torch.empty(x_shape, dtype=dtype, device=dev) if need_x else None, None if dw is None else dw.zero_(),
-                    None if db is None else db.zero_(), None)
-        dy = dy.reshape(rows, N).contiguous()
-        if need_x:
-            g = act8_pack(dy)
-            dx = _fp8_product(g.q, g.scale, rows, qt, scale_t, K, N, None, dtype).view(x_shape)
-        if need_w or need_b:
-            _fp8_wgrad(q, scale, dy, rows, N, K, dw, db)
-        return dx, dw, db, None
+    type ``a`` stands for by default).  Not differentiable: :func:`fp8_linear` is, and states the arithmetic."""
+    if not isinstance(a, Act8) or not isinstance(weight, Fp8Weight):
+        raise TypeError('fp8_matmul: expected an Act8 (act8_pack) and an Fp8Weight (fp8_weight), got %s and %s'
+                        % (type(a).__name__, type(weight).__name__))
+    return _lib.torch_glue().fp8_matmul(a.q, a.scale, a.shape, weight.q, weight.scale, weight.shape, bias, a.dtype if dtype is None else dtype)
 
 
 def fp8_linear(x, weight, bias=None):
-    """x [..., K] times weight [N, K] transposed, plus bias, on 8-bit blocks: y = Q(x) Q(weight)^T + bias, in x's type, fp32 sums.
+    """x [..., K] times weight [N, K] transposed, plus bias, on 8-bit blocks: y = Q(x) Q(weight)^T + bias, in x's type.
 
     ``weight``: a tensor, which is laid out anew on every call (training), or an :class:`Fp8Weight` that the caller keeps
     (inference, or a frozen layer).  Differentiable in x, bias and a weight tensor; Q counts as the identity there:
     dx = Q(dy) Q(weight), dweight = dy^T Q(x), dbias = sum of dy.  The backward pass keeps Q(x), a byte a value, and not x; dy enters
     the weight's gradient unrounded.  Q is the format of :func:`act8_pack`: rows of x and dy in blocks of 128, the weight in blocks
-    of 128 x 128.  Deterministic."""
-    packed = weight if isinstance(weight, Fp8Weight) else None
-    _float_dev('fp8_linear', x, *([weight] if packed is None else []), *([bias] if bias is not None else []))
-    if x.dim() == 0:
-        raise ValueError('fp8_linear: x needs at least one axis')
-    _check_fp8(x.shape[-1], x.device, weight, bias, 'fp8_linear')
-    return _Fp8Linear.apply(x, None if packed is not None else weight, bias, packed)
+    of 128 x 128.  Sums are fp32; for a 16-bit x, y and dx come from the 8-bit matrix instructions, which drop what lies 2^-13 below
+    the largest of eight neighbouring products (2e-5 .. 7e-5 of the result's norm).  Deterministic; no second derivative."""
+    if isinstance(weight, Fp8Weight):
+        return _lib.torch_glue().fp8_linear(x, None, bias, weight.q, weight.scale, weight.qt, weight.scale_t, weight.shape)
+    return _lib.torch_glue().fp8_linear(x, weight, bias, None, None, None, None, ())
 
 
 # --------------------------------------------------------------------------- #

@@ -283,8 +283,10 @@ def test_refuses():
         hip_ops.fp8_matmul(a, w)
     with pytest.raises(TypeError):
         hip_ops.fp8_matmul(a, kept, dtype=torch.int32)
-    with pytest.raises(ValueError):
-        hip_ops.fp8_matmul(hip_ops.act8_pack(x[:, :5]), kept)
+    for call in (lambda: hip_ops.fp8_matmul(hip_ops.act8_pack(x[:, :5]), kept), lambda: hip_ops.fp8_linear(x[:, :5], kept),
+                 lambda: hip_ops.fp8_linear(x, kept, b[:5]), lambda: hip_ops.fp8_matmul(a, kept, b[:5])):
+        with pytest.raises(ValueError):
+            call()
     y = hip_ops.fp8_linear(x.requires_grad_(), w)
     g, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):
