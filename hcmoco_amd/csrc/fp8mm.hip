@@ -31,8 +31,25 @@ struct Mm {
   int split;
 };
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
+// Direct loads from memory to LDS, 16 or 4 bytes a lane: lane l's piece lands at lds + l * BYTES, a piece outside the buffer reads as
+// zero.  In assembly because the compiler, which cannot tell the two stages apart, would wait for the loads of the next stage before
+// every LDS read of this one.  Nothing is written but LDS; whoever reads it waits for vmcnt(0) and a barrier first, and a kernel
+// waits for vmcnt(0) before it ends.
+typedef v4i rsrc_t;
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, int bytes) {
+  const uint64_t a = (uint64_t)p;
+  return rsrc_t{(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xffffu), bytes, 0x00020000};
+}
+template <int BYTES>
+__device__ __forceinline__ void load_lds(rsrc_t r, uint32_t lds, int off) {
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
+constexpr int kOutside = (int)0x80000000;       // an offset past every buffer used here (they are under 2^31 bytes)
 
 // Workgroups go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (whole columns of eight row tiles), so that
 // its L2 serves the rows they share.
@@ -76,19 +93,27 @@ __device__ __forceinline__ void out8(const Mm& P, int m, int n, float (&v)[8]) {
   else store8((_Float16*)P.y + at, left, v);
 }
 
-// BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  Two LDS stages of (BN + BM) x 128 bytes,
-// filled by direct loads; one barrier a block of k.
+// BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  Two LDS stages of (BN + BM) x 128 bytes;
+// one barrier a block of k, behind which the next stage's loads go out between the matrix instructions (all at once they block the
+// waves' LDS reads: 480 -> 431 us at 8192^3).  The 256 x 256 tile is bound by these loads: 64 KB a block of k a CU take 1.4 us when
+// an XCD's workgroups, in step, all wait for the same lines from behind L2, against 1.3 us of matrix instructions and LDS reads.  So
+// each workgroup also touches, two blocks ahead, its share of the lines that the XCD's workgroups will want (431 -> 421 us).
 template <int BN, int BM, int WN, int WM, bool WIDE>
 __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   constexpr int NT = WN * WM * 64, TN = BN / WN / 16, TM = BM / WM / 16;
-  constexpr int LW = BN * 8 / NT, LX = BM * 8 / NT;        // 16-byte pieces a thread moves
+  constexpr int LW = BN * 8 / NT, LX = BM * 8 / NT;        // load instructions of a wave a stage
+  constexpr int PER = (2 * (LW + LX) + TN - 1) / TN;       // of them behind each of the first tiles: all are out at half time
+  constexpr bool TOUCH = BN == 256 && BM == 256;
   static_assert(TN % 2 == 0 && LW >= 1 && LX >= 1 && BN * 8 % NT == 0 && BM * 8 % NT == 0, "tile");
   __shared__ __attribute__((aligned(128))) uint8_t stage[2][(BN + BM) * 128];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wn = wave % WN, wm = wave / WN;
+  __shared__ uint32_t sx_stage[2][BM];                     // the scales of four blocks of k, one dword a row
+  __shared__ uint32_t touched[TOUCH ? 128 : 1];            // never read
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), wn = wave % WN, wm = wave / WN;
   int im, in;
   tile_of(blockIdx.x, (P.M + BM - 1) / BM, (P.N + BN - 1) / BN, im, in);
   const int m0 = im * BM, n0 = in * BN;
-  const int per = (P.kblocks + P.split - 1) / P.split, k_from = blockIdx.z * per, k_to = min(P.kblocks, k_from + per);
+  const int per = ((P.kblocks + P.split - 1) / P.split + 3) & ~3;      // whole dwords of scales
+  const int k_from = blockIdx.z * per, k_to = min(P.kblocks, k_from + per);
 
   const uint8_t* wbase = P.w + (int64_t)n0 * P.ldw;
   const uint8_t* xbase = P.x + (int64_t)m0 * P.ldx;
@@ -97,24 +122,31 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   // Row r of a stage lies at r * 128, its piece c in slot c ^ key(r): eight lanes that read the same piece of eight rows hit eight
   // different slots.  A load instruction of a wave fills eight rows; which piece a lane fetches is what places it.
   const int r8 = lane >> 3, slot = lane & 7;
-  auto issue = [&](int kb, int buf) {
+  rsrc_t rw, rx;
+  int left = 0;
+  auto aim = [&](int kb) {
     const int64_t ko = (int64_t)kb * 128;
-    const rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void*)(wbase + ko), 0, wbytes - (int)ko, 0x00020000);
-    const rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void*)(xbase + ko), 0, xbytes - (int)ko, 0x00020000);
-    const int left = P.ldk - kb * 128;       // pieces past the row's end would be the next row's: sent out of range, they read as zero
-#pragma unroll
-    for (int j = 0; j < LW; ++j) {
+    rw = make_rsrc(wbase + ko, wbytes - (int)ko);
+    rx = make_rsrc(xbase + ko, xbytes - (int)ko);
+    left = P.ldk - kb * 128;       // pieces past the row's end would be the next row's: sent outside, they read as zero
+  };
+  auto issue = [&](int buf, int j) {
+    if (j < LW) {
       const int rg = wave + j * (NT / 64), r = rg * 8 + r8;                     // W rows: key (r & 3) | (r >> 3 & 1) << 2
       const int c = slot ^ ((r8 & 3) | ((rg & 1) << 2));
-      const int off = c * 16 < left ? r * (int)P.ldw + c * 16 : (int)0x80000000;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds_void*)&stage[buf][rg * 1024], 16, off, 0, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < LX; ++j) {
-      const int rg = wave + j * (NT / 64), r = rg * 8 + r8;                     // X rows: key r & 7
+      load_lds<16>(rw, lds_addr(&stage[buf][rg * 1024]), c * 16 < left ? r * (int)P.ldw + c * 16 : kOutside);
+    } else {
+      const int rg = wave + (j - LW) * (NT / 64), r = rg * 8 + r8;              // X rows: key r & 7
       const int c = slot ^ r8;
-      const int off = c * 16 < left ? r * (int)P.ldx + c * 16 : (int)0x80000000;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds_void*)&stage[buf][(BN + rg * 8) * 128], 16, off, 0, 0, 0);
+      load_lds<16>(rx, lds_addr(&stage[buf][(BN + rg * 8) * 128]), c * 16 < left ? r * (int)P.ldx + c * 16 : kOutside);
+    }
+  };
+  const rsrc_t rs = make_rsrc(P.sx + (int64_t)m0 * P.ldsx, (int)(min(P.M - m0, BM) * P.ldsx));
+  auto issue_scales = [&](int kq) {          // blocks 4 kq .. 4 kq + 3; rows past the end read as zero, their sums are not stored
+#pragma unroll
+    for (int j = 0; j < (BM + NT - 1) / NT; ++j) {
+      const int r0 = (wave + j * (NT / 64)) * 64;
+      if (r0 < BM) load_lds<4>(rs, lds_addr(&sx_stage[kq & 1][r0]), (r0 + lane) * (int)P.ldsx + kq * 4);
     }
   };
 
@@ -125,9 +157,6 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   for (int a = 0; a < TN; ++a) wrow[a] = (wn * TN * 16 + 32 * (a >> 1) + (i >> 2) * 8 + (a & 1) * 4 + (i & 3)) * 128 + frag;
 #pragma unroll
   for (int b = 0; b < TM; ++b) xrow[b] = (BN + (wm * TM + b) * 16 + i) * 128 + frag;
-  const uint8_t* sxp[TM];
-#pragma unroll
-  for (int b = 0; b < TM; ++b) sxp[b] = P.sx + (int64_t)min(m0 + (wm * TM + b) * 16 + i, P.M - 1) * P.ldsx;
   const uint8_t* swp = P.sw + (int64_t)(min(n0 + wn * TN * 16, P.N - 1) / 128) * P.ldsw;
 
   v4f acc[TN][TM];
@@ -136,22 +165,39 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
 #pragma unroll
     for (int b = 0; b < TM; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  int sx_next[TM], sw_next = 0;
-  auto scales = [&](int kb) {
+  uint32_t sx4[TM], sw4 = 0, sw_next = 0;
+  if (k_from < k_to) {
+    sw_next = *(const uint32_t*)(swp + k_from);
+    issue_scales(k_from >> 2);
+    aim(k_from);
 #pragma unroll
-    for (int b = 0; b < TM; ++b) sx_next[b] = sxp[b][kb];
-    sw_next = swp[kb];
-  };
-  if (k_from < k_to) scales(k_from), issue(k_from, 0);
+    for (int j = 0; j < LW + LX; ++j) issue(0, j);
+  }
   for (int kb = k_from; kb < k_to; ++kb) {
     const int buf = (kb - k_from) & 1;
-    __builtin_amdgcn_s_waitcnt(0x0f70);          // vmcnt(0): this wave's pieces of the stage have landed
-    __syncthreads();
+    wait_loads();                  // this wave's pieces of the stage have landed
+    __syncthreads();               // everybody's have, and nobody reads the other stage any more
+    if ((kb & 3) == 0) {
+#pragma unroll
+      for (int b = 0; b < TM; ++b) sx4[b] = sx_stage[(kb >> 2) & 1][(wm * TM + b) * 16 + i];
+      sw4 = __builtin_amdgcn_readfirstlane(sw_next);
+    }
+    const bool more = kb + 1 < k_to;
+    if (more && ((kb + 1) & 3) == 0) issue_scales((kb + 1) >> 2), sw_next = *(const uint32_t*)(swp + kb + 1);
+    aim(more ? kb + 1 : kb);
+    if (!more) left = 0;           // nothing follows: the loads below go outside
+    if constexpr (TOUCH) {
+      // of the eight row tiles and four column tiles that run side by side on an XCD: an eighth of this tile's W rows, a quarter of its X rows
+      if (wave < 2 && kb + 2 < k_to) {
+        const int r = wave ? (im & 7) * (BN / 8) + (lane & (BN / 8 - 1)) : (in & 3) * (BM / 4) + (lane & (BM / 4 - 1));
+        if (wave) load_lds<4>(make_rsrc(wbase, wbytes), lds_addr(touched + 64), r * (int)P.ldw + (kb + 2) * 128);
+        else load_lds<4>(make_rsrc(xbase, xbytes), lds_addr(touched), r * (int)P.ldx + (kb + 2) * 128);
+      }
+    }
+    const int sh = (kb & 3) * 8, sw = (sw4 >> sh) & 255;
     int sx[TM];
 #pragma unroll
-    for (int b = 0; b < TM; ++b) sx[b] = sx_next[b];
-    const int sw = sw_next;
-    if (kb + 1 < k_to) scales(kb + 1), issue(kb + 1, buf ^ 1);
+    for (int b = 0; b < TM; ++b) sx[b] = (sx4[b] >> sh) & 255;
     const uint8_t* s = stage[buf];
     v8i xf[TM];
     v8bf xw[WIDE ? TM : 1][4];
@@ -175,8 +221,11 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
         for (int b = 0; b < TM; ++b)
           acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[b], acc[a][b], 0, 0, 0, sw, 0, sx[b]);
       }
+#pragma unroll
+      for (int j = a * PER; j < (a + 1) * PER && j < LW + LX; ++j) issue(buf ^ 1, j);
     }
   }
+  wait_loads();
 #pragma unroll
   for (int b = 0; b < TM; ++b)
 #pragma unroll
@@ -188,15 +237,163 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
     }
 }
 
-// y = sum of the split's partial sums (in order) + bias
-__global__ __launch_bounds__(256) void fp8_join_kernel(const float* __restrict__ part, int split, int64_t n, int N, const void* __restrict__ bias, int bias_dt,
-                                                       void* __restrict__ y, int out_dt) {
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int z = 0; z < split; ++z) s += part[z * n + e];
-    if (bias) s += load_dt(bias, bias_dt, e % N);
-    store_dt(y, out_dt, e, s);
+// A few rows (at most 32): bound by reading W once, and by latency.  Sixteen columns of y a workgroup, the blocks of k dealt to its
+// eight waves, each straight from memory to registers (a W row is read in whole lines: eight waves x 128 bytes); the waves' sums
+// meet in LDS.  X comes packed (T = uint8_t), or as it is and is packed here by every workgroup (at most kFewBlocks blocks of 128: a
+// launch costs more than that); the first workgroup then also writes the packed copy where one is wanted.
+constexpr int kFewRows = 32, kFewBlocks = 256, kFewWaves = 8, kFewAhead = 4;
+
+template <typename T, bool WIDE, int MT>
+__global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(const Mm P, const T* __restrict__ xraw, int64_t ld_raw, int K, uint8_t* __restrict__ q_out,
+                                                                 uint8_t* __restrict__ s_out) {
+  constexpr bool PACK = sizeof(T) > 1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];      // PACK: M rows of (kblocks * 128 + 16) bytes, then M rows of kblocks scales
+  __shared__ float red[kFewWaves][MT * 16][17];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* wr = P.w + (int64_t)min(n0 + i, P.N - 1) * P.ldw;
+  const uint8_t* swr = P.sw + (int64_t)(n0 / 128) * P.ldsw;
+  const v4i zero = {0, 0, 0, 0};
+  auto piece = [&](const uint8_t* row, int at) { return at < P.ldk ? *(const v4i*)(row + at) : zero; };
+
+  v4i wlo[kFewAhead], whi[kFewAhead];
+  int sw[kFewAhead];
+  auto fetch = [&](int u, int kb) {
+    kb = min(kb, P.kblocks - 1);       // past the end: read again, not used
+    wlo[u] = piece(wr, kb * 128 + g * 16);
+    whi[u] = piece(wr, kb * 128 + 64 + g * 16);
+    sw[u] = swr[kb];
+  };
+#pragma unroll
+  for (int u = 0; u < kFewAhead; ++u) fetch(u, wave + u * kFewWaves);
+
+  const int pitch = P.kblocks * 128 + 16;
+  uint8_t* xs = dyn + P.M * pitch;
+  if constexpr (PACK) {
+    const int cells = P.M * P.kblocks;
+    for (int c = t >> 4; c < cells; c += kFewWaves * 4) {
+      const int row = c / P.kblocks, kb = c - row * P.kblocks, col = kb * 128 + (lane & 15) * 8;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (col < K) load8(xraw + (int64_t)row * ld_raw + col, K - col, v);
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+      const int byte = act8_byte(row16_max(m));
+      const v2i b = act8_bytes(v, inv_pow2_of_byte(byte));
+      *(v2i*)(dyn + row * pitch + col) = b;
+      if ((lane & 15) == 0) xs[c] = (uint8_t)byte;
+      if (q_out && blockIdx.x == 0) {
+        if (col < P.ldx) *(v2i*)(q_out + (int64_t)row * P.ldx + col) = b;
+        if ((lane & 15) == 0) s_out[(int64_t)row * P.ldsx + kb] = (uint8_t)byte;
+        else if (kb == P.kblocks - 1 && kb + (lane & 15) < P.ldsx) s_out[(int64_t)row * P.ldsx + kb + (lane & 15)] = 127;
+      }
+    }
+    __syncthreads();
   }
+  v4f acc[MT];
+#pragma unroll
+  for (int b = 0; b < MT; ++b) acc[b] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int base = wave; base < P.kblocks; base += kFewAhead * kFewWaves) {
+#pragma unroll
+    for (int u = 0; u < kFewAhead; ++u) {
+      const int kb = base + u * kFewWaves;
+      if (kb < P.kblocks) {
+        const v8i wf = join16(wlo[u], whi[u]);
+        v8bf ww[4];
+        if constexpr (WIDE) widen(wf, pow2_of_byte(sw[u]), ww);
+#pragma unroll
+        for (int b = 0; b < MT; ++b) {
+          const int row = min(b * 16 + i, P.M - 1);        // rows past the end repeat the last one and are not stored
+          v8i xf;
+          int sx;
+          if constexpr (PACK) {
+            xf = join16(*(const v4i*)(dyn + row * pitch + kb * 128 + g * 16), *(const v4i*)(dyn + row * pitch + kb * 128 + 64 + g * 16));
+            sx = xs[row * P.kblocks + kb];
+          } else {
+            const uint8_t* xr = P.x + (int64_t)row * P.ldx;
+            xf = join16(piece(xr, kb * 128 + g * 16), piece(xr, kb * 128 + 64 + g * 16));
+            sx = P.sx[(int64_t)row * P.ldsx + kb];
+          }
+          if constexpr (WIDE) {
+            v8bf xw[4];
+            widen(xf, pow2_of_byte(sx), xw);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[q], xw[q], acc[b], 0, 0, 0);
+          } else {
+            acc[b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[b], 0, 0, 0, sw[u], 0, sx);
+          }
+        }
+      }
+      fetch(u, kb + kFewAhead * kFewWaves);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < MT; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[wave][b * 16 + i][4 * g + r] = acc[b][r];
+  __syncthreads();
+  for (int e = t; e < MT * 256; e += kFewWaves * 64) {
+    const int m = e >> 4, n = e & 15;
+    if (m >= P.M || n0 + n >= P.N) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int z = 0; z < kFewWaves; ++z) s += red[z][m][n];
+    if (P.bias) s += load_dt(P.bias, P.bias_dt, n0 + n);
+    store_dt(P.y, P.out_dt, (int64_t)m * P.N + n0 + n, s);
+  }
+}
+
+template <typename T, bool WIDE>
+int few(const Mm& P, const T* xraw, int64_t ld_raw, int K, uint8_t* q_out, uint8_t* s_out, hipStream_t st) {
+  const size_t lds = sizeof(T) > 1 ? (size_t)P.M * (P.kblocks * 128 + 16) + (size_t)P.M * P.kblocks : 0;
+  const uint32_t grid = (P.N + 15) / 16;
+  if (P.M <= 16) fp8_few_kernel<T, WIDE, 1><<<grid, kFewWaves * 64, lds, st>>>(P, xraw, ld_raw, K, q_out, s_out);
+  else fp8_few_kernel<T, WIDE, 2><<<grid, kFewWaves * 64, lds, st>>>(P, xraw, ld_raw, K, q_out, s_out);
+  HCM_CHECK_LAUNCH();
+  return 0;
+}
+
+// y (or dW and behind it db) = sum over the split of part[z][e], + bias for y.  SL slices of the split side by side, their sums through LDS:
+// a small output with a deep split would otherwise be a few waves that wait for one load after the other.
+struct Join { const float* part; int split; int64_t stride, n, n2; int N; const void* bias; int bias_dt; void* out; int dt; void* out2; int dt2; };
+
+template <int SL>
+__global__ __launch_bounds__(256) void join_kernel(const Join J) {
+  constexpr int E = 256 / SL;
+  __shared__ float s[SL][E];
+  const int lane = threadIdx.x % E, slice = threadIdx.x / E;
+  const int64_t e = (int64_t)blockIdx.x * E + lane;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (e < J.n + J.n2) {
+    int z = slice;
+    for (; z + 3 * SL < J.split; z += 4 * SL)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a[u] += J.part[(z + u * SL) * J.stride + e];
+    for (; z < J.split; z += SL) a[0] += J.part[z * J.stride + e];
+  }
+  float sum = (a[0] + a[1]) + (a[2] + a[3]);
+  if constexpr (SL > 1) {
+    s[slice][lane] = sum;
+    __syncthreads();
+    if (slice) return;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < SL; ++i) sum += s[i][lane];
+  }
+  if (e < J.n) {
+    if (J.bias) sum += load_dt(J.bias, J.bias_dt, e % J.N);
+    if (J.out) store_dt(J.out, J.dt, e, sum);
+  } else if (e < J.n + J.n2 && J.out2) {
+    store_dt(J.out2, J.dt2, e - J.n, sum);
+  }
+}
+
+int join(const Join& J, hipStream_t st) {
+  const int64_t n = J.n + J.n2;
+  if (J.split >= 16) join_kernel<16><<<(uint32_t)((n + 15) / 16), 256, 0, st>>>(J);
+  else join_kernel<1><<<(uint32_t)((n + 255) / 256), 256, 0, st>>>(J);
+  HCM_CHECK_LAUNCH();
+  return 0;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -212,14 +409,18 @@ struct Wg {
   const void* dy;
   int64_t M;
   int N, K;
-  int rows_per_split;             // a multiple of kWgRows
-  float* part;                    // [split][N * K + N]
+  int64_t rows_per_split;         // a multiple of every kernel's ROWS
+  float* part;                    // split > 1: [split][stride] partial sums, N * K of dW and N of db; else dw, db
+  int64_t stride;
+  void *dw, *db;
+  int dw_dt, db_dt;
 };
 constexpr int kWgRows = 64;
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
+// eight floats -> the bf16 pieces that hold their type exactly
 template <int P>
 __device__ __forceinline__ void pieces(const float (&v)[8], v8bf (&out)[P]) {
   float r[8];
@@ -234,131 +435,189 @@ __device__ __forceinline__ void pieces(const float (&v)[8], v8bf (&out)[P]) {
     }
 }
 
-template <typename T, int P>
-__global__ __launch_bounds__(256) void fp8_wgrad_kernel(const Wg G) {
-  // plane 0: X, planes 1 .. P: the pieces of dy; [kWgRows][128] bf16, 16-byte piece c of row r in slot c ^ swz(r)
-  __shared__ __attribute__((aligned(16))) uint8_t stage[(1 + P) * kWgRows * 256];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wk = wave & 1, wn = wave >> 1;
-  const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
+// TK columns k x TN columns n of dW a workgroup, WK x WN waves; ROWS rows m a stage, two stages.  A thread carries its share of
+// the stage after next in registers while the matrix instructions of this one run; with DIRECT, dy (bf16, rows of 16-byte pieces)
+// goes from memory to LDS by itself, and only X, which is widened on the way, through registers.
+template <typename T, int P, int TK, int TN, int ROWS, int WK, int WN, bool DIRECT>
+__global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
+  constexpr int NT = WK * WN * 64, FA = TK / WK / 16, FB = TN / WN / 16;
+  constexpr int CX = ROWS * TK / 8 / NT, CD = ROWS * TN / 8 / NT;      // pieces of eight values a thread moves
+  constexpr int XBYTES = ROWS * TK * 2, DBYTES = ROWS * TN * 2;
+  static_assert(!DIRECT || (P == 1 && TN == 256 && CD == 4), "direct");
+  static_assert(CX >= 1 && CD >= 1 && NT % (TK / 8) == 0 && NT % (TN / 8) == 0 && kWgRows % ROWS == 0 && TK % 128 == 0, "shape");
+  // X as bf16 [ROWS][TK], then the P pieces of dy [ROWS][TN]; 16-byte piece c of row r in slot c ^ swz(r): the four rows that
+  // sixteen lanes of a transpose read touch lie in different banks
+  __shared__ __attribute__((aligned(16))) uint8_t stage[2][XBYTES + P * DBYTES];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), wk = wave % WK, wn = wave / WK;
+  int ik, in;
+  tile_of(blockIdx.x, (G.K + TK - 1) / TK, (G.N + TN - 1) / TN, ik, in);
+  const int k0 = ik * TK, n0 = in * TN;
   const int64_t m_from = (int64_t)blockIdx.z * G.rows_per_split, m_to = min(G.M, m_from + G.rows_per_split);
   auto swz = [](int r) { return ((r & 3) << 1) | (((r >> 3) & 1) << 3); };
-  // a thread stages a quarter row: 32 values of X and of dy
-  const int sr = t >> 2, sc = (t & 3) * 32;
-  v8i xq;
-  int xs;
-  float d[4][8];
+
+  const int xr = t / (TK / 8), xc = t % (TK / 8), dr = t / (TN / 8), dc = t % (TN / 8);
+  constexpr int XSTEP = NT / (TK / 8), DSTEP = NT / (TN / 8);
+  const bool x_in = k0 + xc * 8 < G.ldq;
+  const int d_left = G.N - (n0 + dc * 8);
+  v2i xq[CX];
+  int xs[CX];
+  typename Vec8<T>::type d[DIRECT ? 1 : CD];
   auto fetch = [&](int64_t m) {
-    const int64_t row = m + sr;
-    const bool in = row < m_to;
-    xq = v8i{0, 0, 0, 0, 0, 0, 0, 0};
-    xs = 127;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < CX; ++j) {
+      const int64_t row = m + xr + j * XSTEP;
+      xq[j] = v2i{0, 0};
+      xs[j] = 127;
+      if (x_in && row < m_to) {
+        xq[j] = *(const v2i*)(G.q + row * G.ldq + k0 + xc * 8);
+        xs[j] = G.scale[row * G.lds + (k0 + xc * 8) / 128];
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[j][i] = 0.f;
-    if (!in) return;
-    const uint8_t* qr = G.q + row * G.ldq + k0 + sc;
-    if (k0 + sc < G.ldq) { const v4i a = *(const v4i*)qr; xq[0] = a[0]; xq[1] = a[1]; xq[2] = a[2]; xq[3] = a[3]; }
-    if (k0 + sc + 16 < G.ldq) { const v4i a = *(const v4i*)(qr + 16); xq[4] = a[0]; xq[5] = a[1]; xq[6] = a[2]; xq[7] = a[3]; }
-    xs = G.scale[row * G.lds + blockIdx.x];
+    for (int j = 0; j < (DIRECT ? 0 : CD); ++j) {
+      const int64_t row = m + dr + j * DSTEP;
+      const T* p = (const T*)G.dy + row * G.N + n0 + dc * 8;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + sc + 8 * j;
-      if (n < G.N) load8((const T*)G.dy + row * G.N + n, G.N - n, d[j]);
+      for (int e = 0; e < 8; ++e) d[j][e] = (T)0.f;
+      if (row < m_to) {
+        if (d_left >= 8) __builtin_memcpy(&d[j], p, 8 * sizeof(T));
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < d_left) d[j][e] = p[e];
+      }
     }
   };
-  auto put = [&]() {
-    const float sf = pow2_of_byte(xs);
+  auto put = [&](int buf) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[8];
-      act8_values(v2i{xq[2 * j], xq[2 * j + 1]}, sf, f);
-      v8bf o[1], e[P];
-      pieces<1>(f, o);
-      const int at = sr * 256 + (((sc >> 3) + j) ^ swz(sr)) * 16;
-      *(v8bf*)(stage + at) = o[0];
-      pieces<P>(d[j], e);
+    for (int j = 0; j < CX; ++j) {
+      const float f = pow2_of_byte(xs[j]);
+      const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][0], f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][0], f, true);
+      const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][1], f, false), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][1], f, true);
+      const int row = xr + j * XSTEP;
+      *(v8bf*)(stage[buf] + row * TK * 2 + ((xc ^ swz(row)) << 4)) = v8bf{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+    }
 #pragma unroll
-      for (int p = 0; p < P; ++p) *(v8bf*)(stage + (1 + p) * kWgRows * 256 + at) = e[p];
+    for (int j = 0; j < (DIRECT ? 0 : CD); ++j) {
+      const int row = dr + j * DSTEP, at = XBYTES + row * TN * 2 + ((dc ^ swz(row)) << 4);
+      if constexpr (P == 1) {
+        *(v8bf*)(stage[buf] + at) = __builtin_bit_cast(v8bf, d[j]);
+      } else {
+        float v[8];
+        v8bf e[P];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (float)d[j][q];
+        pieces<P>(v, e);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *(v8bf*)(stage[buf] + at + p * DBYTES) = e[p];
+      }
     }
   };
-  v4f acc[4][4], accb[4];
+  // DIRECT: rows 2 (wave + 8 j), + 1 of the stage that begins at m; columns past the row's end are another row's, in sums that are not stored
+  auto direct = [&](int64_t m, int buf) {
+    const rsrc_t rd = make_rsrc((const T*)G.dy + m * G.N + n0, (int)(min(m_to - m, (int64_t)ROWS) * G.N - n0) * 2);
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    accb[a] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int b = 0; b < 4; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int j = 0; j < CD; ++j) {
+      const int row = 2 * (wave + 8 * j) + (lane >> 5);
+      load_lds<16>(rd, lds_addr(stage[buf] + XBYTES + 2 * (wave + 8 * j) * TN * 2), row * G.N * 2 + (((lane & 31) ^ swz(row)) << 4));
+    }
+  };
   const int p16 = lane & 15, g = lane >> 4;
-  // eight rows 32 s + 8 g .. + 7 of sixteen columns from c0 (a multiple of 16), lane p16 the column
-  auto frag = [&](int plane, int s, int c0) {
+  // rows 32 s + 8 g .. + 7 of sixteen columns from c0 (a multiple of 16), lane p16 the column; `plane`: LDS, rows of `width` values
+  auto frag = [&](const uint8_t* plane, int width, int s, int c0) {
     v4s h[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int r = 32 * s + 8 * g + 4 * u + (p16 >> 2), c = c0 + 4 * (p16 & 3);
-      h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(stage + plane * kWgRows * 256 + r * 256 + (((c >> 3) ^ swz(r)) << 4) + (c & 7) * 2));
+      h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(plane + r * width * 2 + (((c >> 3) ^ swz(r)) << 4) + (c & 7) * 2));
     }
     return __builtin_bit_cast(v8bf, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  const bool sums = blockIdx.x == 0 && wk == 0;
+
+  v4f acc[FA][FB], accb[FB];
+#pragma unroll
+  for (int b = 0; b < FB; ++b) {
+    accb[b] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int a = 0; a < FA; ++a) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool sums = ik == 0 && wk == 0;        // these waves also sum dy's columns: a product with ones
   v8bf ones;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (__bf16)1.f;
-  if (m_from < m_to) fetch(m_from);
-  for (int64_t m = m_from; m < m_to; m += kWgRows) {
-    put();
-    __syncthreads();
-    if (m + kWgRows < m_to) fetch(m + kWgRows);
+  for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
+
+  if (m_from < m_to) {
+    if constexpr (DIRECT) direct(m_from, 0);
+    fetch(m_from);
+    put(0);
+    fetch(m_from + ROWS);          // rows past the split's end come as zeros, without a load
+  }
+  if constexpr (DIRECT) wait_loads();
+  __syncthreads();
+  int buf = 0;
+  for (int64_t m = m_from; m < m_to; m += ROWS, buf ^= 1) {
+    if (m + ROWS < m_to) {
+      if constexpr (DIRECT) direct(m + ROWS, buf ^ 1);
+      put(buf ^ 1);
+      fetch(m + 2 * ROWS);
+    }
 #pragma unroll
-    for (int s = 0; s < kWgRows / 32; ++s) {
-      v8bf xf[4];
+    for (int s = 0; s < ROWS / 32; ++s) {
+      v8bf xf[FA];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) xf[a] = frag(0, s, wk * 64 + a * 16);
+      for (int a = 0; a < FA; ++a) xf[a] = frag(stage[buf], TK, s, (wk * FA + a) * 16);
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const v8bf df = frag(1 + p, s, wn * 64 + b * 16);
+        for (int b = 0; b < FB; ++b) {
+          const v8bf df = frag(stage[buf] + XBYTES + p * DBYTES, TN, s, (wn * FB + b) * 16);
 #pragma unroll
-          for (int a = 0; a < 4; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[a], df, acc[a][b], 0, 0, 0);
+          for (int a = 0; a < FA; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[a], df, acc[a][b], 0, 0, 0);
           if (sums) accb[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, df, accb[b], 0, 0, 0);
         }
     }
+    if constexpr (DIRECT) wait_loads();
     __syncthreads();
   }
-  float* out = G.part + (int64_t)blockIdx.z * ((int64_t)G.N * G.K + G.N);
+  float* part = G.part ? G.part + blockIdx.z * G.stride : nullptr;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const int n = n0 + wn * 64 + b * 16 + p16;
+  for (int b = 0; b < FB; ++b) {
+    const int n = n0 + (wn * FB + b) * 16 + p16;
     if (n >= G.N) continue;
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int k = k0 + wk * 64 + a * 16 + 4 * g;
+    for (int a = 0; a < FA; ++a) {
+      const int k = k0 + (wk * FA + a) * 16 + 4 * g;
+      const int64_t at = (int64_t)n * G.K + k;
+      if (part && k + 4 <= G.K) {
+        __builtin_memcpy(part + at, &acc[a][b], 16);
+      } else if (!part && G.dw && G.dw_dt == kF32 && k + 4 <= G.K) {
+        __builtin_memcpy((float*)G.dw + at, &acc[a][b], 16);
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (k + r < G.K) out[(int64_t)n * G.K + k + r] = acc[a][b][r];
+        for (int r = 0; r < 4; ++r)
+          if (k + r < G.K) {
+            if (part) part[at + r] = acc[a][b][r];
+            else if (G.dw) store_dt(G.dw, G.dw_dt, at + r, acc[a][b][r]);
+          }
+      }
     }
-    if (sums && g == 0) out[(int64_t)G.N * G.K + n] = accb[b][0];
+    if (sums && g == 0) {
+      if (part) part[(int64_t)G.N * G.K + n] = accb[b][0];
+      else if (G.db) store_dt(G.db, G.db_dt, n, accb[b][0]);
+    }
   }
 }
 
-// dW = sum of the split's partial sums, db likewise behind them
-__global__ __launch_bounds__(256) void fp8_wgrad_join_kernel(const float* __restrict__ part, int split, int64_t n, int N, void* __restrict__ dw, int dw_dt,
-                                                             void* __restrict__ db, int db_dt) {
-  const int64_t all = n + N;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int z = 0; z < split; ++z) s += part[z * all + e];
-    if (e < n) { if (dw) store_dt(dw, dw_dt, e, s); }
-    else if (db) store_dt(db, db_dt, e - n, s);
-  }
-}
-
-int wgrad_split(int64_t M, int N, int K) {
-  const int64_t tiles = (int64_t)((N + 127) / 128) * ((K + 127) / 128), steps = (M + kWgRows - 1) / kWgRows;
-  int64_t split = (512 + tiles - 1) / tiles;
+// The tile of dW: 256 x 256 where that leaves enough workgroups and dy can go to LDS directly (bf16, rows of 16-byte pieces), else 128 x 128; 256 x 128 for two or three pieces.
+struct WgPlan { int tk, tn, split; };
+WgPlan wgrad_plan(int64_t M, int N, int K, int dy_dt) {
+  auto tiles = [&](int tk, int tn) { return (int64_t)((K + tk - 1) / tk) * ((N + tn - 1) / tn); };
+  WgPlan p = dy_dt != kBF16 ? WgPlan{256, 128, 1} : tiles(256, 256) >= 64 && N % 8 == 0 ? WgPlan{256, 256, 1} : WgPlan{128, 128, 1};
+  const int64_t have = tiles(p.tk, p.tn), want = p.tn == 256 ? 256 : 512, steps = (M + kWgRows - 1) / kWgRows;
+  int64_t split = have >= want / 2 ? 1 : want / have;
   if (split > (steps + 7) / 8) split = (steps + 7) / 8;      // at least 512 rows each
-  return (int)(split < 1 ? 1 : split);
+  p.split = (int)split;
+  return p;
 }
 
 struct Plan { int tile, split; };      // tile: columns = rows of a workgroup's tile
@@ -381,7 +640,7 @@ Plan plan(int M, int N, int kblocks, bool wide) {
 extern "C" {
 
 size_t hcm_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= kFewRows || N <= 0 || K <= 0) return 0;
   const Plan p = plan(M, N, (K + 127) / 128, out_dtype == kF32);
   return p.split > 1 ? (size_t)p.split * M * N * sizeof(float) : 0;
 }
@@ -391,15 +650,17 @@ int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
                    size_t workspace_bytes, hcm_stream_t stream) {
   if (!x || !x_scale || !w || !w_scale || !y || M <= 0 || M > INT32_MAX - 512 || N <= 0 || N > (1 << 22) || K <= 0 || K > (1 << 22) || ldx != hcm_act8_pitch(K) || ldw != ldx ||
       ldsx != hcm_act8_scale_pitch(K) || ldsw != ldsx || out_dtype < 0 || out_dtype > 2 || (bias && (bias_dtype < 0 || bias_dtype > 2)) ||
-      ((uintptr_t)x & 15) || ((uintptr_t)w & 15))
+      ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || ((uintptr_t)x_scale & 3) || ((uintptr_t)w_scale & 3))
     return (int)hipErrorInvalidValue;
   Mm P = {x, x_scale, w, w_scale, ldx, ldsx, ldw, ldsw, M, N, (K + 127) / 128, (int)ldx, bias, bias_dtype, out_dtype, y, nullptr, 1};
   const bool wide = out_dtype == kF32;
+  hipStream_t st = (hipStream_t)stream;
+  if (M <= kFewRows)
+    return wide ? few<uint8_t, true>(P, nullptr, 0, K, nullptr, nullptr, st) : few<uint8_t, false>(P, nullptr, 0, K, nullptr, nullptr, st);
   const Plan p = plan(M, N, P.kblocks, wide);
   if (workspace_bytes < hcm_fp8_matmul_workspace_bytes(M, N, K, out_dtype) || (p.split > 1 && !workspace)) return (int)hipErrorInvalidValue;
   P.split = p.split;
   if (p.split > 1) P.part = (float*)workspace;
-  hipStream_t st = (hipStream_t)stream;
   const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((N + p.tile - 1) / p.tile);
   if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
   const dim3 grid((uint32_t)tiles, 1, p.split);
@@ -410,36 +671,56 @@ int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   else fp8_tile_kernel<64, 64, 2, 2, false><<<grid, 256, 0, st>>>(P);
   HCM_CHECK_LAUNCH();
   if (p.split > 1) {
-    const int64_t n = (int64_t)M * N, blocks = (n + 255) / 256;
-    fp8_join_kernel<<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(P.part, p.split, n, N, bias, bias_dtype, y, out_dtype);
-    HCM_CHECK_LAUNCH();
+    const int64_t n = (int64_t)M * N;
+    return join({P.part, p.split, n, n, 0, N, bias, bias_dtype, y, out_dtype, nullptr, 0}, st);
   }
   return 0;
 }
 
-size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K) {
+int hcm_fp8_rows_supported(int64_t M, int K) { return M > 0 && M <= kFewRows && K > 0 && K <= (1 << 22) && M * ((K + 127) / 128) <= kFewBlocks; }
+
+int hcm_fp8_rows(const void* x, int dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const uint8_t* w_scale, int64_t ldsw, const void* bias,
+                 int bias_dtype, int M, int N, int K, void* y, uint8_t* q, uint8_t* q_scale, hcm_stream_t stream) {
+  if (!x || !w || !w_scale || !y || !hcm_fp8_rows_supported(M, K) || N <= 0 || N > (1 << 22) || ldx < K || ldw != hcm_act8_pitch(K) ||
+      ldsw != hcm_act8_scale_pitch(K) || dtype < 0 || dtype > 2 || (bias && (bias_dtype < 0 || bias_dtype > 2)) || (!q != !q_scale) ||
+      ((uintptr_t)w & 15) || ((uintptr_t)q & 15))
+    return (int)hipErrorInvalidValue;
+  const Mm P = {nullptr, nullptr, w, w_scale, ldw, ldsw, ldw, ldsw, M, N, (K + 127) / 128, (int)ldw, bias, bias_dtype, dtype, y, nullptr, 1};
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == kF32) return few<float, true>(P, (const float*)x, ldx, K, q, q_scale, st);
+  if (dtype == kBF16) return few<__bf16, false>(P, (const __bf16*)x, ldx, K, q, q_scale, st);
+  return few<_Float16, false>(P, (const _Float16*)x, ldx, K, q, q_scale, st);
+}
+
+// partial sums of dW and db, a multiple of four floats apart
+static int64_t wgrad_stride(int N, int K) { return ((int64_t)N * K + N + 3) / 4 * 4; }
+
+size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K, int dy_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return (size_t)wgrad_split(M, N, K) * ((size_t)N * K + N) * sizeof(float);
+  const WgPlan p = wgrad_plan(M, N, K, dy_dtype);
+  return p.split > 1 ? (size_t)p.split * wgrad_stride(N, K) * sizeof(float) : 0;
 }
 
 int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldsx, const void* dy, int dy_dtype, int64_t M, int N, int K, void* dw,
                   int dw_dtype, void* db, int db_dtype, void* workspace, size_t workspace_bytes, hcm_stream_t stream) {
-  if (!x || !x_scale || !dy || (!dw && !db) || !workspace || M <= 0 || M >= (1ll << 31) || N <= 0 || K <= 0 || K > (1 << 22) || N > (1 << 22) ||
+  if (!x || !x_scale || !dy || (!dw && !db) || M <= 0 || M >= (1ll << 31) || N <= 0 || K <= 0 || K > (1 << 22) || N > (1 << 22) ||
       ldx != hcm_act8_pitch(K) || ldsx != hcm_act8_scale_pitch(K) || dy_dtype < 0 || dy_dtype > 2 || dw_dtype < 0 || dw_dtype > 2 || db_dtype < 0 ||
-      db_dtype > 2 || ((uintptr_t)x & 15) || workspace_bytes < hcm_fp8_wgrad_workspace_bytes(M, N, K))
+      db_dtype > 2 || ((uintptr_t)x & 15) || ((uintptr_t)dy & 15))
     return (int)hipErrorInvalidValue;
-  const int split = wgrad_split(M, N, K);
-  const int64_t steps = (M + kWgRows - 1) / kWgRows;
-  const Wg G = {x, x_scale, ldx, ldsx, dy, M, N, K, (int)((steps + split - 1) / split * kWgRows), (float*)workspace};
-  const dim3 grid((K + 127) / 128, (N + 127) / 128, split);
+  const WgPlan p = wgrad_plan(M, N, K, dy_dtype);
+  if (p.split > 1 && (!workspace || workspace_bytes < hcm_fp8_wgrad_workspace_bytes(M, N, K, dy_dtype))) return (int)hipErrorInvalidValue;
+  const int64_t tiles = (int64_t)((K + p.tk - 1) / p.tk) * ((N + p.tn - 1) / p.tn), steps = (M + kWgRows - 1) / kWgRows;
+  if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
+  const Wg G = {x,  x_scale, ldx, ldsx, dy, M, N, K, (steps + p.split - 1) / p.split * kWgRows, p.split > 1 ? (float*)workspace : nullptr, wgrad_stride(N, K),
+                dw, db,      dw_dtype, db_dtype};
+  const dim3 grid((uint32_t)tiles, 1, p.split);
   hipStream_t st = (hipStream_t)stream;
-  if (dy_dtype == kF32) fp8_wgrad_kernel<float, 3><<<grid, 256, 0, st>>>(G);
-  else if (dy_dtype == kBF16) fp8_wgrad_kernel<__bf16, 1><<<grid, 256, 0, st>>>(G);
-  else fp8_wgrad_kernel<_Float16, 2><<<grid, 256, 0, st>>>(G);
+  if (dy_dtype == kF32) fp8_wgrad_kernel<float, 3, 256, 128, 32, 4, 2, false><<<grid, 512, 0, st>>>(G);
+  else if (dy_dtype == kF16) fp8_wgrad_kernel<_Float16, 2, 256, 128, 32, 4, 2, false><<<grid, 512, 0, st>>>(G);
+  else if (p.tn == 256) fp8_wgrad_kernel<__bf16, 1, 256, 256, 64, 2, 4, true><<<grid, 512, 0, st>>>(G);
+  else fp8_wgrad_kernel<__bf16, 1, 128, 128, 64, 2, 2, false><<<grid, 256, 0, st>>>(G);
   HCM_CHECK_LAUNCH();
-  const int64_t n = (int64_t)N * K, blocks = (n + N + 255) / 256;
-  fp8_wgrad_join_kernel<<<(uint32_t)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(G.part, split, n, N, dw, dw_dtype, db, db_dtype);
-  HCM_CHECK_LAUNCH();
+  if (p.split > 1) return join({G.part, p.split, G.stride, (int64_t)N * K, N, N, nullptr, 0, dw, dw_dtype, db, db_dtype}, st);
   return 0;
 }
 

@@ -275,13 +275,30 @@ Tensor fp8_matmul(const Tensor& q, const Tensor& scale, at::IntArrayRef shape, c
   return product({q, scale}, M, wq, ws, N, K, b, with_last(shape, N), dtype);
 }
 
+// Q(x) W^T + bias for x as it comes; `packed`: Q(x) is wanted too
+Tensor linear_forward(const Rows& r, const Tensor& wq, const Tensor& ws, int64_t N, const Tensor& bias, at::IntArrayRef shape, Packed* packed) {
+  if (!hcm_fp8_rows_supported(r.rows, r.cols)) {
+    Packed a = pack_raw(r, "fp8_linear");
+    Tensor y = product(a, r.rows, wq, ws, N, r.cols, bias, shape, r.t.scalar_type());
+    if (packed) *packed = a;
+    return y;
+  }
+  Packed a;
+  if (packed) a = *packed = packed_buffers(r.rows, r.cols, r.t);
+  Tensor y = at::empty(shape, r.t.options());
+  check_rc(hcm_fp8_rows(r.t.data_ptr(), dt_of(r.t, "fp8_linear"), r.ld, bytes(wq), wq.size(1), bytes(ws), ws.size(1), ptr(bias), dt_of(bias, "fp8_linear"),
+                        (int)r.rows, (int)N, r.cols, y.data_ptr(), bytes(a.q), bytes(a.scale), stream_of(r.t)),
+           "hcm_fp8_rows");
+  return y;
+}
+
 struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Tensor& wq, const Tensor& ws,
                         const Tensor& wqt, const Tensor& wst, int64_t N) {
     const Tensor w = value(weight), b = value(bias);
     const Rows r = rows_of(x, "fp8_linear");
-    const Packed a = pack_raw(r, "fp8_linear");
-    Tensor y = product(a, r.rows, wq, ws, N, r.cols, b, with_last(x.sizes(), N), x.scalar_type());
+    Packed a;
+    Tensor y = linear_forward(r, wq, ws, N, b, with_last(x.sizes(), N), &a);
     // x itself is not kept: the 8-bit operand of this product is the checkpoint that the weight's gradient reads
     ctx->save_for_backward({a.q, a.scale, wqt, wst});
     ctx->saved_data["m"] = std::vector<int64_t>{r.rows, N, r.cols, wants_grad(x), wants_grad(w), wants_grad(b),
@@ -299,16 +316,14 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     Tensor dx, dw, db;
     {
       at::AutoGradMode off(false);
-      const Tensor dy = grads[0].contiguous();
+      Tensor dy = grads[0].contiguous();
+      if ((uintptr_t)dy.data_ptr() & 15) dy = dy.clone();        // a view that begins anywhere: hcm_fp8_wgrad reads 16-byte pieces
       const c10::DeviceGuard guard(dy.device());
       if (nw) dw = at::empty({N, K}, dy.options().dtype((at::ScalarType)m[6]));
       if (nb) db = at::empty({N}, dy.options().dtype((at::ScalarType)m[7]));
-      if (nx) {
-        const Packed g = pack_raw({dy, M, N, (int)N}, "fp8_linear");
-        dx = product(g, M, saved[2], saved[3], K, N, Tensor(), shape, dy.scalar_type());
-      }
+      if (nx) dx = linear_forward({dy, M, N, (int)N}, saved[2], saved[3], K, Tensor(), shape, nullptr);
       if ((nw || nb) && M) {
-        const size_t n = hcm_fp8_wgrad_workspace_bytes(M, (int)N, (int)K);
+        const size_t n = hcm_fp8_wgrad_workspace_bytes(M, (int)N, (int)K, dt_of(dy, "fp8_linear"));
         const Tensor work = workspace(n, dy);
         check_rc(hcm_fp8_wgrad(bytes(saved[0]), saved[0].size(1), bytes(saved[1]), saved[1].size(1), dy.data_ptr(), dt_of(dy, "fp8_linear"), M, (int)N,
                                (int)K, ptr(dw), dt_of(dw, "fp8_linear"), ptr(db), dt_of(db, "fp8_linear"), ptr(work), n, stream_of(dy)),
@@ -349,8 +364,7 @@ Tensor fp8_linear(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   }
   TORCH_CHECK_VALUE(x.numel() / K <= INT32_MAX - 512, "fp8_linear: too many rows");
   if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) {
-    const Rows r = rows_of(x, "fp8_linear");
-    return product(pack_raw(r, "fp8_linear"), r.rows, wq, ws, N, K, b, with_last(x.sizes(), N), x.scalar_type());
+    return linear_forward(rows_of(x, "fp8_linear"), wq, ws, N, b, with_last(x.sizes(), N), nullptr);
   }
   return Fp8Linear::apply(x, weight, bias, wq, ws, wqt, wst, N);
 }

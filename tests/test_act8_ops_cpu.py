@@ -66,18 +66,26 @@ def test_products_refuse():
     good = dict(x=P, ldx=272, sx=P, ldsx=4, w=P, ldw=272, sw=P, ldsw=4, b=Z, bd=0, M=4, N=200, K=270, y=P, od=0, ws=P, n=1 << 30)
     for bad in (dict(x=Z), dict(ldx=270), dict(sx=Z), dict(ldsx=3), dict(w=Z), dict(ldw=288), dict(sw=Z), dict(ldsw=8), dict(b=P, bd=3), dict(M=0),
                 dict(M=2 ** 31 - 1), dict(N=0), dict(N=2 ** 22 + 1), dict(K=0), dict(K=2 ** 22 + 1), dict(y=Z), dict(od=-1), dict(od=3),
-                dict(x=C.c_void_p(4104)), dict(w=C.c_void_p(4104))):
+                dict(x=C.c_void_p(4104)), dict(w=C.c_void_p(4104)), dict(sx=C.c_void_p(4097)), dict(sw=C.c_void_p(4098))):
         a = {**good, **bad}
         assert L.hcm_fp8_matmul(*[a[k] for k in good], Z) != 0, bad
-    need = L.hcm_fp8_matmul_workspace_bytes(32, 128, 4096, 0)
+    need = L.hcm_fp8_matmul_workspace_bytes(64, 128, 4096, 0)
     assert need > 0 and L.hcm_fp8_matmul_workspace_bytes(8192, 8192, 8192, 1) == 0 and L.hcm_fp8_matmul_workspace_bytes(0, 1, 1, 0) == 0
-    a = {**good, **dict(ldx=4096, ldw=4096, ldsx=32, ldsw=32, M=32, N=128, K=4096)}
+    a = {**good, **dict(ldx=4096, ldw=4096, ldsx=32, ldsw=32, M=64, N=128, K=4096)}
     for bad in (dict(n=need - 1), dict(ws=Z)):
         assert L.hcm_fp8_matmul(*[{**a, **bad}[k] for k in good], Z) != 0, bad
-    need = L.hcm_fp8_wgrad_workspace_bytes(1000, 200, 270)
-    good = dict(x=P, ldx=272, sx=P, ldsx=4, dy=P, dd=0, M=1000, N=200, K=270, dw=P, wd=0, db=P, bd=0, ws=P, n=need)
+    good = dict(x=P, dt=0, ldx=270, w=P, ldw=272, sw=P, ldsw=4, b=Z, bd=0, M=4, N=200, K=270, y=P, q=Z, s=Z)
+    for bad in (dict(x=Z), dict(dt=3), dict(ldx=269), dict(w=Z), dict(ldw=270), dict(sw=Z), dict(ldsw=3), dict(b=P, bd=4), dict(M=0), dict(M=33),
+                dict(N=0), dict(K=0), dict(y=Z), dict(q=P), dict(s=P), dict(w=C.c_void_p(4100)), dict(q=C.c_void_p(4100), s=P),
+                dict(M=9, K=3712, ldx=3712, ldw=3712, ldsw=32)):
+        a = {**good, **bad}
+        assert L.hcm_fp8_rows(*[a[k] for k in good], Z) != 0, bad
+    assert [L.hcm_fp8_rows_supported(*a) for a in ((1, 32768), (1, 32769), (32, 1024), (32, 1025), (33, 1), (0, 1))] == [1, 0, 1, 0, 0, 0]
+    need = L.hcm_fp8_wgrad_workspace_bytes(4000, 200, 270, 0)
+    assert need > 0 and L.hcm_fp8_wgrad_workspace_bytes(8192, 4096, 4096, 1) == 0
+    good = dict(x=P, ldx=272, sx=P, ldsx=4, dy=P, dd=0, M=4000, N=200, K=270, dw=P, wd=0, db=P, bd=0, ws=P, n=need)
     for bad in (dict(x=Z), dict(ldx=270), dict(sx=Z), dict(ldsx=2), dict(dy=Z), dict(dd=3), dict(M=0), dict(M=2 ** 31), dict(N=0), dict(K=0),
-                dict(N=2 ** 22 + 1), dict(dw=Z, db=Z), dict(wd=9), dict(bd=-1), dict(ws=Z), dict(n=need - 1), dict(x=C.c_void_p(4104))):
+                dict(N=2 ** 22 + 1), dict(dw=Z, db=Z), dict(wd=9), dict(bd=-1), dict(ws=Z), dict(n=need - 1), dict(x=C.c_void_p(4104)), dict(dy=C.c_void_p(4104))):
         a = {**good, **bad}
         assert L.hcm_fp8_wgrad(*[a[k] for k in good], Z) != 0, bad
 

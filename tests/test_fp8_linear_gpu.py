@@ -81,10 +81,21 @@ def test_training_step(M, N, K, dtype):
     _check_step(x, w, b, dy, _run(x, w, b, dy))
 
 
-@pytest.mark.parametrize('M,N,K', [(3500, 3600, 300), (1800, 1900, 200), (3000, 100, 1300), (40, 4000, 700)])
+@pytest.mark.parametrize('M,N,K', [(3500, 3600, 300), (1800, 1900, 200), (3000, 100, 1300), (40, 4000, 700), (1000, 2040, 2049), (333, 2100, 2300),
+                                   (4200, 264, 1900)])
 def test_every_tile_and_split(M, N, K):
     x, w, b, dy = _inputs(M, N, K, torch.bfloat16, 7)
     _check_step(x, w, None, dy, _run(x, w, None, dy))
+
+
+def test_gradient_that_begins_anywhere():
+    from hcmoco_amd import hip_ops
+    x, w, b, dy = _inputs(300, 96, 200, torch.bfloat16, 6)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    y = hip_ops.fp8_linear(*leaves)
+    room = torch.zeros(300 * 96 + 1, dtype=torch.bfloat16, device=DEV)
+    room[1:] = dy.flatten().to(DEV)
+    _check_step(x, w, b, dy, [y.detach()] + list(torch.autograd.grad(y, leaves, room[1:].view(300, 96))))
 
 
 def test_many_rows_few_columns():
