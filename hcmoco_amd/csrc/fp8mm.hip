@@ -13,6 +13,7 @@
 // a 16-bit y (2^-9, 2^-12), and it is over that of an fp32 one, so y in fp32 takes the WIDE form: the 8-bit values are widened to bf16
 // on their way from LDS -- exact, the scales included, by v_cvt_scalef32_pk_bf16_fp8 -- and multiplied by v_mfma_f32_16x16x32_bf16,
 // whose sums are fp32 (1e-8 .. 3e-7 on the same data), at half the rate.
+#include <cmath>
 #include "act8.h"
 #include "../../include/hcmoco_hip.h"
 
@@ -48,7 +49,12 @@ __device__ __forceinline__ void load_lds(rsrc_t r, uint32_t lds, int off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
+// All but the newest N loads of this wave are done, and all of its LDS reads: before a barrier behind which others overwrite what it read.
+template <int N = 0>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "vmcnt");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);      // vmcnt(N) lgkmcnt(0)
+}
 constexpr int kOutside = (int)0x80000000;       // an offset past every buffer used here (they are under 2^31 bytes)
 
 // Workgroups go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (whole columns of eight row tiles), so that
@@ -93,20 +99,21 @@ __device__ __forceinline__ void out8(const Mm& P, int m, int n, float (&v)[8]) {
   else store8((_Float16*)P.y + at, left, v);
 }
 
-// BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  Two LDS stages of (BN + BM) x 128 bytes;
-// one barrier a block of k, behind which the next stage's loads go out between the matrix instructions (all at once they block the
-// waves' LDS reads: 480 -> 431 us at 8192^3).  The 256 x 256 tile is bound by these loads: 64 KB a block of k a CU take 1.4 us when
+// BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  S LDS stages of (BN + BM) x 128 bytes in a ring;
+// one barrier a block of k, behind which the loads of the stage S - 1 blocks ahead go out between the matrix instructions (all at once
+// they block the waves' LDS reads: 480 -> 431 us at 8192^3).  Small tiles run where few workgroups do and a block of k is latency: four
+// stages.  The 256 x 256 tile is bound by these loads: 64 KB a block of k a CU take 1.4 us when
 // an XCD's workgroups, in step, all wait for the same lines from behind L2, against 1.3 us of matrix instructions and LDS reads.  So
 // each workgroup also touches, two blocks ahead, its share of the lines that the XCD's workgroups will want (431 -> 421 us).
-template <int BN, int BM, int WN, int WM, bool WIDE>
+template <int BN, int BM, int WN, int WM, int S, bool WIDE>
 __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   constexpr int NT = WN * WM * 64, TN = BN / WN / 16, TM = BM / WM / 16;
   constexpr int LW = BN * 8 / NT, LX = BM * 8 / NT;        // load instructions of a wave a stage
   constexpr int PER = (2 * (LW + LX) + TN - 1) / TN;       // of them behind each of the first tiles: all are out at half time
   constexpr bool TOUCH = BN == 256 && BM == 256;
   static_assert(TN % 2 == 0 && LW >= 1 && LX >= 1 && BN * 8 % NT == 0 && BM * 8 % NT == 0, "tile");
-  __shared__ __attribute__((aligned(128))) uint8_t stage[2][(BN + BM) * 128];
-  __shared__ uint32_t sx_stage[2][BM];                     // the scales of four blocks of k, one dword a row
+  __shared__ __attribute__((aligned(128))) uint8_t stage[S][(BN + BM) * 128];
+  __shared__ uint32_t sx_stage[2][BM], sw_stage[2][64];    // the scales of four blocks of k, one dword a row of X, one a block of W
   __shared__ uint32_t touched[TOUCH ? 128 : 1];            // never read
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), wn = wave % WN, wm = wave / WN;
   int im, in;
@@ -142,12 +149,15 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
     }
   };
   const rsrc_t rs = make_rsrc(P.sx + (int64_t)m0 * P.ldsx, (int)(min(P.M - m0, BM) * P.ldsx));
+  const int wblocks = (min(P.N - n0, BN) + 127) / 128;
+  const rsrc_t rsw = make_rsrc(P.sw + (int64_t)(n0 / 128) * P.ldsw, wblocks * (int)P.ldsw);
   auto issue_scales = [&](int kq) {          // blocks 4 kq .. 4 kq + 3; rows past the end read as zero, their sums are not stored
 #pragma unroll
     for (int j = 0; j < (BM + NT - 1) / NT; ++j) {
       const int r0 = (wave + j * (NT / 64)) * 64;
       if (r0 < BM) load_lds<4>(rs, lds_addr(&sx_stage[kq & 1][r0]), (r0 + lane) * (int)P.ldsx + kq * 4);
     }
+    if (wave == NT / 64 - 1) load_lds<4>(rsw, lds_addr(sw_stage[kq & 1]), lane < wblocks ? lane * (int)P.ldsw + kq * 4 : kOutside);
   };
 
   const int i = lane & 15, g = lane >> 4;
@@ -157,35 +167,37 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   for (int a = 0; a < TN; ++a) wrow[a] = (wn * TN * 16 + 32 * (a >> 1) + (i >> 2) * 8 + (a & 1) * 4 + (i & 3)) * 128 + frag;
 #pragma unroll
   for (int b = 0; b < TM; ++b) xrow[b] = (BN + (wm * TM + b) * 16 + i) * 128 + frag;
-  const uint8_t* swp = P.sw + (int64_t)(min(n0 + wn * TN * 16, P.N - 1) / 128) * P.ldsw;
-
   v4f acc[TN][TM];
 #pragma unroll
   for (int a = 0; a < TN; ++a)
 #pragma unroll
     for (int b = 0; b < TM; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  uint32_t sx4[TM], sw4 = 0, sw_next = 0;
-  if (k_from < k_to) {
-    sw_next = *(const uint32_t*)(swp + k_from);
-    issue_scales(k_from >> 2);
-    aim(k_from);
+  uint32_t sx4[TM], sw4 = 0;
+  auto begin = [&](int kb) {       // what comes before the loads of block kb's stage; past the end they go outside
+    if (kb < k_to && (kb & 3) == 0) issue_scales(kb >> 2);
+    aim(min(kb, k_to - 1));
+    if (kb >= k_to) left = 0;
+  };
+  if (k_from < k_to)
+    for (int p = 0; p < S - 1; ++p) {
+      begin(k_from + p);
 #pragma unroll
-    for (int j = 0; j < LW + LX; ++j) issue(0, j);
-  }
-  for (int kb = k_from; kb < k_to; ++kb) {
-    const int buf = (kb - k_from) & 1;
-    wait_loads();                  // this wave's pieces of the stage have landed
-    __syncthreads();               // everybody's have, and nobody reads the other stage any more
+      for (int j = 0; j < LW + LX; ++j) issue(p, j);
+    }
+  int buf = 0;
+  for (int kb = k_from; kb < k_to; ++kb, buf = buf + 1 == S ? 0 : buf + 1) {
+    wait_loads<(S - 2) * (LW + LX)>();       // this wave's pieces of the stage have landed (its scales went out before them)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();            // everybody's have, and nobody reads the stage before it any more
+    asm volatile("" ::: "memory");
     if ((kb & 3) == 0) {
 #pragma unroll
       for (int b = 0; b < TM; ++b) sx4[b] = sx_stage[(kb >> 2) & 1][(wm * TM + b) * 16 + i];
-      sw4 = __builtin_amdgcn_readfirstlane(sw_next);
+      sw4 = __builtin_amdgcn_readfirstlane(sw_stage[(kb >> 2) & 1][wn * TN * 16 / 128]);
     }
-    const bool more = kb + 1 < k_to;
-    if (more && ((kb + 1) & 3) == 0) issue_scales((kb + 1) >> 2), sw_next = *(const uint32_t*)(swp + kb + 1);
-    aim(more ? kb + 1 : kb);
-    if (!more) left = 0;           // nothing follows: the loads below go outside
+    begin(kb + S - 1);
+    const int next = buf == 0 ? S - 1 : buf - 1;
     if constexpr (TOUCH) {
       // of the eight row tiles and four column tiles that run side by side on an XCD: an eighth of this tile's W rows, a quarter of its X rows
       if (wave < 2 && kb + 2 < k_to) {
@@ -222,7 +234,7 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
           acc[a][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf[b], acc[a][b], 0, 0, 0, sw, 0, sx[b]);
       }
 #pragma unroll
-      for (int j = a * PER; j < (a + 1) * PER && j < LW + LX; ++j) issue(buf ^ 1, j);
+      for (int j = a * PER; j < (a + 1) * PER && j < LW + LX; ++j) issue(next, j);
     }
   }
   wait_loads();
@@ -435,16 +447,16 @@ __device__ __forceinline__ void pieces(const float (&v)[8], v8bf (&out)[P]) {
     }
 }
 
-// TK columns k x TN columns n of dW a workgroup, WK x WN waves; ROWS rows m a stage, two stages.  A thread carries its share of
-// the stage after next in registers while the matrix instructions of this one run; with DIRECT, dy (bf16, rows of 16-byte pieces)
-// goes from memory to LDS by itself, and only X, which is widened on the way, through registers.
+// TK columns k x TN columns n of dW a workgroup of WK x WN = 8 waves; ROWS rows m a stage, two stages.  What a stage needs is on its
+// way in registers AHEAD stages before it goes to LDS (one stage of a small tile computes in 0.3 us, and a load takes 1 - 2 us; a second
+// set does not fit the registers of the 384-wide tile: 75.6 against 65.6 us for 131072 x 128 x 270).  With
+// DIRECT, dy (bf16, rows of 16-byte pieces) goes from memory to LDS by itself, and only X, which is widened on the way, through registers.
 template <typename T, int P, int TK, int TN, int ROWS, int WK, int WN, bool DIRECT>
-__global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
-  constexpr int NT = WK * WN * 64, FA = TK / WK / 16, FB = TN / WN / 16;
-  constexpr int CX = ROWS * TK / 8 / NT, CD = ROWS * TN / 8 / NT;      // pieces of eight values a thread moves
+__global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
+  constexpr int FA = TK / WK / 16, FB = TN / WN / 16, AHEAD = DIRECT || TK == 384 ? 1 : 2;
+  constexpr int RG = ROWS / 32, CX = TK / 128 * RG, CD = DIRECT ? 4 : RG;      // pieces a thread moves: eight values, sixteen threads a row of 128
   constexpr int XBYTES = ROWS * TK * 2, DBYTES = ROWS * TN * 2;
-  static_assert(!DIRECT || (P == 1 && TN == 256 && CD == 4), "direct");
-  static_assert(CX >= 1 && CD >= 1 && NT % (TK / 8) == 0 && NT % (TN / 8) == 0 && kWgRows % ROWS == 0 && TK % 128 == 0, "shape");
+  static_assert(WK * WN == 8 && TK % 128 == 0 && kWgRows % ROWS == 0 && (DIRECT ? P == 1 && TN == 256 && ROWS == 64 : TN == 128), "shape");
   // X as bf16 [ROWS][TK], then the P pieces of dy [ROWS][TN]; 16-byte piece c of row r in slot c ^ swz(r): the four rows that
   // sixteen lanes of a transpose read touch lie in different banks
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][XBYTES + P * DBYTES];
@@ -455,58 +467,60 @@ __global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
   const int64_t m_from = (int64_t)blockIdx.z * G.rows_per_split, m_to = min(G.M, m_from + G.rows_per_split);
   auto swz = [](int r) { return ((r & 3) << 1) | (((r >> 3) & 1) << 3); };
 
-  const int xr = t / (TK / 8), xc = t % (TK / 8), dr = t / (TN / 8), dc = t % (TN / 8);
-  constexpr int XSTEP = NT / (TK / 8), DSTEP = NT / (TN / 8);
-  const bool x_in = k0 + xc * 8 < G.ldq;
-  const int d_left = G.N - (n0 + dc * 8);
-  v2i xq[CX];
-  int xs[CX];
-  typename Vec8<T>::type d[DIRECT ? 1 : CD];
-  auto fetch = [&](int64_t m) {
+  const int tr = t >> 4, tc = t & 15;
+  const int x_off = tr * (int)G.ldq + k0 + tc * 8, x_left = (int)G.ldq - k0 - tc * 8, s_off = tr * (int)G.lds + k0 / 128;
+  struct Set { v2i xq[CX]; int xs[CX]; typename Vec8<T>::type d[DIRECT ? 1 : CD]; };
+  Set set[AHEAD];
+  float cs[DIRECT ? 1 : 8] = {};       // of the columns tc * 8 .. + 7 of dy, this thread's rows
+  auto d_at = [&](int64_t m, int j) { return (m + tr + j * 32) * G.N + n0 + tc * 8; };
+  // The stage that begins at m.  Rows of X past the split's end read as zero; of dy they are made zero in put().
+  auto fetch = [&](Set& S, int64_t m) {
+    const int rows = (int)max((int64_t)0, min(m_to - m, (int64_t)ROWS));
+    const auto rq = __builtin_amdgcn_make_buffer_rsrc((void*)(G.q + m * G.ldq), 0, rows * (int)G.ldq, 0x00020000);
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(G.scale + m * G.lds), 0, rows * (int)G.lds, 0x00020000);
 #pragma unroll
     for (int j = 0; j < CX; ++j) {
-      const int64_t row = m + xr + j * XSTEP;
-      xq[j] = v2i{0, 0};
-      xs[j] = 127;
-      if (x_in && row < m_to) {
-        xq[j] = *(const v2i*)(G.q + row * G.ldq + k0 + xc * 8);
-        xs[j] = G.scale[row * G.lds + (k0 + xc * 8) / 128];
-      }
+      const int panel = j / RG, row = j % RG * 32;
+      S.xq[j] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(
+                                            rq, panel * 128 < x_left ? x_off + row * (int)G.ldq + panel * 128 : kOutside, 0, 0));
+      S.xs[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, s_off + row * (int)G.lds + panel, 0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < (DIRECT ? 0 : CD); ++j) {
-      const int64_t row = m + dr + j * DSTEP;
-      const T* p = (const T*)G.dy + row * G.N + n0 + dc * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d[j][e] = (T)0.f;
-      if (row < m_to) {
-        if (d_left >= 8) __builtin_memcpy(&d[j], p, 8 * sizeof(T));
-        else
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < d_left) d[j][e] = p[e];
-      }
-    }
+    for (int j = 0; j < (DIRECT ? 0 : CD) && G.M * G.N >= 8; ++j)        // unconditional: a load in a branch would be waited for at the branch's end
+      __builtin_memcpy(&S.d[j], (const T*)G.dy + max((int64_t)0, min(d_at(m, j), G.M * G.N - 8)), 8 * sizeof(T));
   };
-  auto put = [&](int buf) {
+  auto put = [&](Set& S, int buf, int64_t m) {
 #pragma unroll
     for (int j = 0; j < CX; ++j) {
-      const float f = pow2_of_byte(xs[j]);
-      const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][0], f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][0], f, true);
-      const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][1], f, false), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[j][1], f, true);
-      const int row = xr + j * XSTEP;
-      *(v8bf*)(stage[buf] + row * TK * 2 + ((xc ^ swz(row)) << 4)) = v8bf{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
+      const float f = pow2_of_byte(S.xs[j]);
+      const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(S.xq[j][0], f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(S.xq[j][0], f, true);
+      const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(S.xq[j][1], f, false), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(S.xq[j][1], f, true);
+      const int row = tr + j % RG * 32, chunk = j / RG * 16 + tc;
+      *(v8bf*)(stage[buf] + row * TK * 2 + ((chunk ^ swz(row)) << 4)) = v8bf{a[0], a[1], b[0], b[1], c[0], c[1], e[0], e[1]};
     }
 #pragma unroll
     for (int j = 0; j < (DIRECT ? 0 : CD); ++j) {
-      const int row = dr + j * DSTEP, at = XBYTES + row * TN * 2 + ((dc ^ swz(row)) << 4);
+      const int row = tr + j * 32, at = XBYTES + row * TN * 2 + ((tc ^ swz(row)) << 4);
+      // columns past N are whatever lies there: their sums are not stored
+      const int64_t from = d_at(m, j);
+      if (m + row >= m_to) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) S.d[j][q] = (T)0.f;
+      } else if (from + 8 > G.M * G.N) {                 // the last values of dy: fetch() read others, so as not to pass its end
+#pragma unroll
+        for (int q = 0; q < 8; ++q) S.d[j][q] = from + q < G.M * G.N ? ((const T*)G.dy)[from + q] : (T)0.f;
+      }
+      if (!DIRECT && ik == 0) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) cs[DIRECT ? 0 : q] += (float)S.d[j][q];
+      }
       if constexpr (P == 1) {
-        *(v8bf*)(stage[buf] + at) = __builtin_bit_cast(v8bf, d[j]);
+        *(v8bf*)(stage[buf] + at) = __builtin_bit_cast(v8bf, S.d[j]);
       } else {
         float v[8];
         v8bf e[P];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = (float)d[j][q];
+        for (int q = 0; q < 8; ++q) v[q] = (float)S.d[j][q];
         pieces<P>(v, e);
 #pragma unroll
         for (int p = 0; p < P; ++p) *(v8bf*)(stage[buf] + at + p * DBYTES) = e[p];
@@ -534,32 +548,25 @@ __global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
     return __builtin_bit_cast(v8bf, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  v4f acc[FA][FB], accb[FB];
+  v4f acc[FA][FB], accb[DIRECT ? FB : 1];
 #pragma unroll
   for (int b = 0; b < FB; ++b) {
-    accb[b] = v4f{0.f, 0.f, 0.f, 0.f};
+    accb[DIRECT ? b : 0] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int a = 0; a < FA; ++a) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-  const bool sums = ik == 0 && wk == 0;        // these waves also sum dy's columns: a product with ones
+  // the first column of tiles also sums dy's columns: as a product with ones where a thread never sees dy
+  const bool sums = DIRECT && ik == 0 && wk == 0;
   v8bf ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (__bf16)1.f;
 
-  if (m_from < m_to) {
-    if constexpr (DIRECT) direct(m_from, 0);
-    fetch(m_from);
-    put(0);
-    fetch(m_from + ROWS);          // rows past the split's end come as zeros, without a load
-  }
-  if constexpr (DIRECT) wait_loads();
-  __syncthreads();
-  int buf = 0;
-  for (int64_t m = m_from; m < m_to; m += ROWS, buf ^= 1) {
+  // the stage at m is in `buf`, the next ones in `S` and (AHEAD = 2) the other set
+  auto step = [&](Set& S, int buf, int64_t m) {
     if (m + ROWS < m_to) {
       if constexpr (DIRECT) direct(m + ROWS, buf ^ 1);
-      put(buf ^ 1);
-      fetch(m + 2 * ROWS);
+      put(S, buf ^ 1, m + ROWS);
+      fetch(S, m + (1 + AHEAD) * ROWS);
     }
 #pragma unroll
     for (int s = 0; s < ROWS / 32; ++s) {
@@ -573,11 +580,24 @@ __global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
           const v8bf df = frag(stage[buf] + XBYTES + p * DBYTES, TN, s, (wn * FB + b) * 16);
 #pragma unroll
           for (int a = 0; a < FA; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[a], df, acc[a][b], 0, 0, 0);
-          if (sums) accb[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, df, accb[b], 0, 0, 0);
+          if (sums) accb[DIRECT ? b : 0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, df, accb[DIRECT ? b : 0], 0, 0, 0);
         }
     }
     if constexpr (DIRECT) wait_loads();
     __syncthreads();
+  };
+  if (m_from < m_to) {
+    if constexpr (DIRECT) direct(m_from, 0);
+    fetch(set[0], m_from);
+    if constexpr (AHEAD == 2) fetch(set[1], m_from + ROWS);
+    put(set[0], 0, m_from);
+    fetch(set[0], m_from + AHEAD * ROWS);
+  }
+  if constexpr (DIRECT) wait_loads();
+  __syncthreads();
+  for (int64_t m = m_from; m < m_to; m += 2 * ROWS) {
+    step(set[AHEAD - 1], 0, m);
+    if (m + ROWS < m_to) step(set[0], 1, m + ROWS);
   }
   float* part = G.part ? G.part + blockIdx.z * G.stride : nullptr;
 #pragma unroll
@@ -602,22 +622,61 @@ __global__ __launch_bounds__(WK * WN * 64) void fp8_wgrad_kernel(const Wg G) {
       }
     }
     if (sums && g == 0) {
-      if (part) part[(int64_t)G.N * G.K + n] = accb[b][0];
-      else if (G.db) store_dt(G.db, G.db_dt, n, accb[b][0]);
+      if (part) part[(int64_t)G.N * G.K + n] = accb[DIRECT ? b : 0][0];
+      else if (G.db) store_dt(G.db, G.db_dt, n, accb[DIRECT ? b : 0][0]);
+    }
+  }
+  if (!DIRECT && ik == 0) {
+    float* red = (float*)stage;        // [8][128]; the last step ended with a barrier
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      float v = cs[DIRECT ? 0 : q];
+      v += __shfl_xor(v, 16, 64);
+      v += __shfl_xor(v, 32, 64);
+      if (lane < 16) red[wave * 128 + tc * 8 + q] = v;
+    }
+    __syncthreads();
+    if (t < 128 && n0 + t < G.N) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v += red[w * 128 + t];
+      if (part) part[(int64_t)G.N * G.K + n0 + t] = v;
+      else if (G.db) store_dt(G.db, G.db_dt, n0 + t, v);
     }
   }
 }
 
-// The tile of dW: 256 x 256 where that leaves enough workgroups and dy can go to LDS directly (bf16, rows of 16-byte pieces), else 128 x 128; 256 x 128 for two or three pieces.
+// The tile of dW: 256 x 256 where that leaves enough workgroups and dy can go to LDS directly (bf16, rows of 16-byte pieces).  Else 128
+// columns n, and of 384, 256 or 128 columns k those that pad K least (K = 270: 384; 131072 rows of fp32, N = 128).
 struct WgPlan { int tk, tn, split; };
 WgPlan wgrad_plan(int64_t M, int N, int K, int dy_dt) {
   auto tiles = [&](int tk, int tn) { return (int64_t)((K + tk - 1) / tk) * ((N + tn - 1) / tn); };
-  WgPlan p = dy_dt != kBF16 ? WgPlan{256, 128, 1} : tiles(256, 256) >= 64 && N % 8 == 0 ? WgPlan{256, 256, 1} : WgPlan{128, 128, 1};
-  const int64_t have = tiles(p.tk, p.tn), want = p.tn == 256 ? 256 : 512, steps = (M + kWgRows - 1) / kWgRows;
-  int64_t split = have >= want / 2 ? 1 : want / have;
-  if (split > (steps + 7) / 8) split = (steps + 7) / 8;      // at least 512 rows each
+  auto padded = [&](int tk) { return (int64_t)(K + tk - 1) / tk * tk; };
+  WgPlan p = {384, 128, 1};
+  if (dy_dt == kBF16 && N % 8 == 0 && tiles(256, 256) >= 64) p = {256, 256, 1};
+  else if (padded(256) < padded(384) || padded(128) < padded(384)) p.tk = padded(256) <= padded(128) ? 256 : 128;
+  // A stage of 64 rows costs about 2 us where few workgroups run, a split's partial sums N K 8 bytes at 4 TB/s: sqrt of the ratio,
+  // as long as the workgroups it makes find a free CU.
+  const int64_t have = tiles(p.tk, p.tn), want = p.tk == 128 ? 512 : 256, steps = (M + kWgRows - 1) / kWgRows;
+  int64_t split = (int64_t)ceil(sqrt((double)steps * 1e6 / ((double)N * K)));
+  if (split > want / have) split = want / have;
+  if (split > steps) split = steps;
+  if (split < 1) split = 1;
   p.split = (int)split;
   return p;
+}
+
+template <typename T, int P, int ROWS>
+void wgrad(const WgPlan& p, const dim3& grid, const Wg& G, hipStream_t st) {
+  if (p.tk == 384) fp8_wgrad_kernel<T, P, 384, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
+  else if (p.tk == 256) fp8_wgrad_kernel<T, P, 256, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
+  else fp8_wgrad_kernel<T, P, 128, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
+}
+
+template <int TILE, int S>
+void tile_launch(bool wide, const dim3& grid, const Mm& P, hipStream_t st) {
+  if (wide) fp8_tile_kernel<TILE, TILE, 2, 2, S, true><<<grid, 256, 0, st>>>(P);
+  else fp8_tile_kernel<TILE, TILE, 2, 2, S, false><<<grid, 256, 0, st>>>(P);
 }
 
 struct Plan { int tile, split; };      // tile: columns = rows of a workgroup's tile
@@ -664,11 +723,12 @@ int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((N + p.tile - 1) / p.tile);
   if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
   const dim3 grid((uint32_t)tiles, 1, p.split);
-  if (p.tile == 256) fp8_tile_kernel<256, 256, 2, 4, false><<<grid, 512, 0, st>>>(P);
-  else if (p.tile == 128 && wide) fp8_tile_kernel<128, 128, 2, 2, true><<<grid, 256, 0, st>>>(P);
-  else if (p.tile == 128) fp8_tile_kernel<128, 128, 2, 2, false><<<grid, 256, 0, st>>>(P);
-  else if (wide) fp8_tile_kernel<64, 64, 2, 2, true><<<grid, 256, 0, st>>>(P);
-  else fp8_tile_kernel<64, 64, 2, 2, false><<<grid, 256, 0, st>>>(P);
+  // Four stages keep a long contraction fed where few workgroups run (500 x 4096 x 4096: 21.8 -> 17.4 us); a short one has no use for
+  // them, and two stages leave room for a second workgroup on the CU (131072 x 128 x 270 in fp32: 41.7 -> 30.6 us).
+  const bool deep = P.kblocks > 4;
+  if (p.tile == 256) fp8_tile_kernel<256, 256, 2, 4, 2, false><<<grid, 512, 0, st>>>(P);
+  else if (p.tile == 128) deep ? tile_launch<128, 4>(wide, grid, P, st) : tile_launch<128, 2>(wide, grid, P, st);
+  else deep ? tile_launch<64, 4>(wide, grid, P, st) : tile_launch<64, 2>(wide, grid, P, st);
   HCM_CHECK_LAUNCH();
   if (p.split > 1) {
     const int64_t n = (int64_t)M * N;
@@ -715,10 +775,10 @@ int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t
                 dw, db,      dw_dtype, db_dtype};
   const dim3 grid((uint32_t)tiles, 1, p.split);
   hipStream_t st = (hipStream_t)stream;
-  if (dy_dtype == kF32) fp8_wgrad_kernel<float, 3, 256, 128, 32, 4, 2, false><<<grid, 512, 0, st>>>(G);
-  else if (dy_dtype == kF16) fp8_wgrad_kernel<_Float16, 2, 256, 128, 32, 4, 2, false><<<grid, 512, 0, st>>>(G);
+  if (dy_dtype == kF32) wgrad<float, 3, 32>(p, grid, G, st);
+  else if (dy_dtype == kF16) wgrad<_Float16, 2, 32>(p, grid, G, st);
   else if (p.tn == 256) fp8_wgrad_kernel<__bf16, 1, 256, 256, 64, 2, 4, true><<<grid, 512, 0, st>>>(G);
-  else fp8_wgrad_kernel<__bf16, 1, 128, 128, 64, 2, 2, false><<<grid, 256, 0, st>>>(G);
+  else wgrad<__bf16, 1, 64>(p, grid, G, st);
   HCM_CHECK_LAUNCH();
   if (p.split > 1) return join({G.part, p.split, G.stride, (int64_t)N * K, N, N, nullptr, 0, dw, dw_dtype, db, db_dtype}, st);
   return 0;
