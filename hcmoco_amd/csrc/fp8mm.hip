@@ -5,7 +5,7 @@
 // A block of 128 along k is ONE scaled matrix instruction (v_mfma_scale_f32_16x16x128_f8f6f4), and the format's scale byte is
 // its scale operand: the scales cost no arithmetic.  Its two operands only have to agree on the order of k, so a lane takes
 // the 16-byte pieces g and g + 4 of its row (g = lane / 16).  W is the A operand, so that a lane ends up with neighbouring
-// columns of y; the sixteen A rows of two instructions are interleaved so that they are eight neighbours.
+// columns of y: four, a 16-byte piece of fp32 (WIDE); for a 16-bit y the A rows of two instructions are interleaved so that they are eight.
 //
 // Precision.  Every 8-bit matrix instruction of this chip adds its products in groups of eight neighbouring k, aligned to the
 // group's largest product, and drops what lies below 2^-13 of it (measured on single products, the same for the scaled form and for
@@ -99,6 +99,23 @@ __device__ __forceinline__ void out8(const Mm& P, int m, int n, float (&v)[8]) {
   else store8((_Float16*)P.y + at, left, v);
 }
 
+// four neighbouring columns of one row, fp32
+__device__ __forceinline__ void out4(const Mm& P, int m, int n, v4f v) {
+  const int left = P.N - n;
+  if (m >= P.M || left <= 0) return;
+  float* y = P.part ? P.part + ((int64_t)blockIdx.z * P.M + m) * P.N + n : (float*)P.y + (int64_t)m * P.N + n;
+  if (left >= 4) {
+    if (P.bias && !P.part)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += load_dt(P.bias, P.bias_dt, n + r);
+    __builtin_memcpy(y, &v, 16);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < left) y[r] = v[r] + (P.bias && !P.part ? load_dt(P.bias, P.bias_dt, n + r) : 0.f);
+  }
+}
+
 // BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  S LDS stages of (BN + BM) x 128 bytes in a ring;
 // one barrier a block of k, behind which the loads of the stage S - 1 blocks ahead go out between the matrix instructions (all at once
 // they block the waves' LDS reads: 480 -> 431 us at 8192^3).  Small tiles run where few workgroups do and a block of k is latency: four
@@ -139,8 +156,8 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   };
   auto issue = [&](int buf, int j) {
     if (j < LW) {
-      const int rg = wave + j * (NT / 64), r = rg * 8 + r8;                     // W rows: key (r & 3) | (r >> 3 & 1) << 2
-      const int c = slot ^ ((r8 & 3) | ((rg & 1) << 2));
+      const int rg = wave + j * (NT / 64), r = rg * 8 + r8;                     // W rows: key (r & 3) | (r >> 3 & 1) << 2, WIDE r & 7
+      const int c = slot ^ (WIDE ? r8 : (r8 & 3) | ((rg & 1) << 2));
       load_lds<16>(rw, lds_addr(&stage[buf][rg * 1024]), c * 16 < left ? r * (int)P.ldw + c * 16 : kOutside);
     } else {
       const int rg = wave + (j - LW) * (NT / 64), r = rg * 8 + r8;              // X rows: key r & 7
@@ -164,7 +181,7 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   const int frag = (g ^ (i & 7)) << 4;
   int wrow[TN], xrow[TM];
 #pragma unroll
-  for (int a = 0; a < TN; ++a) wrow[a] = (wn * TN * 16 + 32 * (a >> 1) + (i >> 2) * 8 + (a & 1) * 4 + (i & 3)) * 128 + frag;
+  for (int a = 0; a < TN; ++a) wrow[a] = (wn * TN * 16 + (WIDE ? a * 16 + i : 32 * (a >> 1) + (i >> 2) * 8 + (a & 1) * 4 + (i & 3))) * 128 + frag;
 #pragma unroll
   for (int b = 0; b < TM; ++b) xrow[b] = (BN + (wm * TM + b) * 16 + i) * 128 + frag;
   v4f acc[TN][TM];
@@ -238,6 +255,13 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
     }
   }
   wait_loads();
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int b = 0; b < TM; ++b)
+#pragma unroll
+      for (int a = 0; a < TN; ++a) out4(P, m0 + (wm * TM + b) * 16 + i, n0 + (wn * TN + a) * 16 + 4 * g, acc[a][b]);
+    return;
+  }
 #pragma unroll
   for (int b = 0; b < TM; ++b)
 #pragma unroll
