@@ -480,7 +480,7 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
   constexpr int FA = TK / WK / 16, FB = TN / WN / 16, AHEAD = DIRECT || TK == 384 ? 1 : 2;
   constexpr int RG = ROWS / 32, CX = TK / 128 * RG, CD = DIRECT ? 4 : RG;      // pieces a thread moves: eight values, sixteen threads a row of 128
   constexpr int XBYTES = ROWS * TK * 2, DBYTES = ROWS * TN * 2;
-  static_assert(WK * WN == 8 && TK % 128 == 0 && kWgRows % ROWS == 0 && (DIRECT ? P == 1 && TN == 256 && ROWS == 64 : TN == 128), "shape");
+  static_assert(WK * WN == 8 && TK % 128 == 0 && kWgRows % ROWS == 0 && (DIRECT ? P == 1 && TN == 256 && ROWS == 64 && FB == CD : TN == 128), "shape");
   // X as bf16 [ROWS][TK], then the P pieces of dy [ROWS][TN]; 16-byte piece c of row r in slot c ^ swz(r): the four rows that
   // sixteen lanes of a transpose read touch lie in different banks
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][XBYTES + P * DBYTES];
@@ -551,14 +551,11 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
       }
     }
   };
-  // DIRECT: rows 2 (wave + 8 j), + 1 of the stage that begins at m; columns past the row's end are another row's, in sums that are not stored
-  auto direct = [&](int64_t m, int buf) {
+  // DIRECT: rows 2 (wave + 8 j), + 1 of the stage that begins at m, one load instruction; columns past the row's end are another row's, in sums that are not stored
+  auto direct = [&](int64_t m, int buf, int j) {
     const rsrc_t rd = make_rsrc((const T*)G.dy + m * G.N + n0, (int)(min(m_to - m, (int64_t)ROWS) * G.N - n0) * 2);
-#pragma unroll
-    for (int j = 0; j < CD; ++j) {
-      const int row = 2 * (wave + 8 * j) + (lane >> 5);
-      load_lds<16>(rd, lds_addr(stage[buf] + XBYTES + 2 * (wave + 8 * j) * TN * 2), row * G.N * 2 + (((lane & 31) ^ swz(row)) << 4));
-    }
+    const int row = 2 * (wave + 8 * j) + (lane >> 5);
+    load_lds<16>(rd, lds_addr(stage[buf] + XBYTES + 2 * (wave + 8 * j) * TN * 2), row * G.N * 2 + (((lane & 31) ^ swz(row)) << 4));
   };
   const int p16 = lane & 15, g = lane >> 4;
   // rows 32 s + 8 g .. + 7 of sixteen columns from c0 (a multiple of 16), lane p16 the column; `plane`: LDS, rows of `width` values
@@ -588,7 +585,6 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
   // the stage at m is in `buf`, the next ones in `S` and (AHEAD = 2) the other set
   auto step = [&](Set& S, int buf, int64_t m) {
     if (m + ROWS < m_to) {
-      if constexpr (DIRECT) direct(m + ROWS, buf ^ 1);
       put(S, buf ^ 1, m + ROWS);
       fetch(S, m + (1 + AHEAD) * ROWS);
     }
@@ -605,13 +601,18 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
 #pragma unroll
           for (int a = 0; a < FA; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[a], df, acc[a][b], 0, 0, 0);
           if (sums) accb[DIRECT ? b : 0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, df, accb[DIRECT ? b : 0], 0, 0, 0);
+          // between the instructions: all at once they hold up the LDS reads (8192 x 4096 x 4096: 273 -> 246 us)
+          if constexpr (DIRECT)
+            if (s == 0 && m + ROWS < m_to) direct(m + ROWS, buf ^ 1, b);
         }
     }
     if constexpr (DIRECT) wait_loads();
     __syncthreads();
   };
   if (m_from < m_to) {
-    if constexpr (DIRECT) direct(m_from, 0);
+    if constexpr (DIRECT)
+#pragma unroll
+      for (int j = 0; j < CD; ++j) direct(m_from, 0, j);
     fetch(set[0], m_from);
     if constexpr (AHEAD == 2) fetch(set[1], m_from + ROWS);
     put(set[0], 0, m_from);

@@ -102,6 +102,7 @@ Packed pack_raw(const Rows& r, const char* name) {
 
 std::tuple<Tensor, Tensor> act8_pack(const Tensor& x) {
   check_float(x, x, "act8_pack");
+  at::AutoGradMode off(false);
   const c10::DeviceGuard guard(x.device());
   Packed p = pack_raw(rows_of(x, "act8_pack"), "act8_pack");
   return {p.q, p.scale};

@@ -721,7 +721,6 @@ class Act8:
         return self.q.numel() + self.scale.numel()
 
 
-@torch.no_grad()
 def act8_pack(x):
     """``x`` [..., C] (float32 / bfloat16 / float16) -> :class:`Act8`: a byte a value and a byte for 128 of them.  The largest
     relative error of a value within 2^14 of its block's largest is 2^-4 (half an e4m3 step); what lies further below is held to
@@ -731,7 +730,6 @@ def act8_pack(x):
     return Act8(q, scale, x.shape, x.dtype)
 
 
-@torch.no_grad()
 def act8_unpack(p, dtype=None):
     """The tensor an :class:`Act8` stands for, as ``dtype`` (its own by default), clamped to the type's largest finite value."""
     if not isinstance(p, Act8):
@@ -765,13 +763,11 @@ class Fp8Weight:
         return self.q.numel() + self.scale.numel() + self.qt.numel() + self.scale_t.numel()
 
 
-@torch.no_grad()
 def fp8_weight(weight):
     """``weight`` [N, K] (float32 / bfloat16 / float16) -> :class:`Fp8Weight`, laid out once for any number of products."""
     return Fp8Weight(*_lib.torch_glue().fp8_weight(weight), weight.shape, weight.dtype)
 
 
-@torch.no_grad()
 def fp8_matmul(a, weight, bias=None, dtype=None):
     """``a`` (:class:`Act8`, [..., K]) times ``weight`` (:class:`Fp8Weight`, [N, K]) transposed, plus ``bias``: [..., N] as ``dtype`` (the
     type ``a`` stands for by default).  Not differentiable: :func:`fp8_linear` is, and states the arithmetic."""
