@@ -35,7 +35,8 @@ struct Mm {
 // Direct loads from memory to LDS, 16 or 4 bytes a lane: lane l's piece lands at lds + l * BYTES, a piece outside the buffer reads as
 // zero.  In assembly because the compiler, which cannot tell the two stages apart, would wait for the loads of the next stage before
 // every LDS read of this one.  Nothing is written but LDS; whoever reads it waits for vmcnt(0) and a barrier first, and a kernel
-// waits for vmcnt(0) before it ends.
+// waits for vmcnt(0) before it ends.  (s_nop 4: the wait states between a vector instruction that writes a scalar register, which may stand
+// right before, and a load that takes its buffer from it; the compiler does not look for them in here.)
 typedef v4i rsrc_t;
 __device__ __forceinline__ rsrc_t make_rsrc(const void* p, int bytes) {
   const uint64_t a = (uint64_t)p;
@@ -44,9 +45,9 @@ __device__ __forceinline__ rsrc_t make_rsrc(const void* p, int bytes) {
 template <int BYTES>
 __device__ __forceinline__ void load_lds(rsrc_t r, uint32_t lds, int off) {
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 // All but the newest N loads of this wave are done, and all of its LDS reads: before a barrier behind which others overwrite what it read.

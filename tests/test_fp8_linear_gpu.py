@@ -157,10 +157,15 @@ def test_scales_span_the_range():
     w[:, 128:256] *= 2.0 ** -70
     w[128:] *= 2.0 ** 20
     x[3] = 0
-    want, mag = _mm(held8(x)[0], held8(w, 128)[0])
-    y = hip_ops.fp8_linear(x.to(DEV), hip_ops.fp8_weight(w.to(DEV)))
-    _close(y, want, _sum_tol(512, torch.float32) * mag, torch.float32, 'y')
-    assert (y[3] == 0).all()
+    for rows in (20, 200):                              # the kernel for a few rows, and the tiles
+        x = x.repeat(rows // 20, 1)
+        want, mag = _mm(held8(x)[0], held8(w, 128)[0])
+        y = hip_ops.fp8_linear(x.to(DEV), hip_ops.fp8_weight(w.to(DEV)))
+        _close(y, want, _sum_tol(512, torch.float32) * mag, torch.float32, 'y')
+        assert (y[3] == 0).all()
+        x16 = x.to(torch.bfloat16)                      # (bf16 has fp32's range)
+        want, mag = _mm(held8(x16)[0], held8(w, 128)[0])
+        _close(hip_ops.fp8_linear(x16.to(DEV), hip_ops.fp8_weight(w.to(DEV))), want, _sum_tol(512, torch.bfloat16) * mag, torch.bfloat16, 'y16')
 
 
 def test_rows_that_are_not_finite_stay_by_themselves():
@@ -175,6 +180,52 @@ def test_rows_that_are_not_finite_stay_by_themselves():
         keep = torch.ones(M, dtype=torch.bool)
         keep[[2, 8]] = False
         assert torch.equal(y[keep], clean[keep]) and y[~keep].isnan().all()
+
+
+def test_packed_rows_are_the_checkpoint():
+    """A few rows are packed inside the product's kernel, more of them by act8_pack: the weight's gradient reads the same bytes."""
+    from hcmoco_amd import hip_ops
+    for M, K in ((3, 270), (32, 1024), (32, 1025), (33, 270)):
+        x, w, b, dy = _inputs(M, 40, K, torch.bfloat16, M + K)
+        xs, ws = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        y = hip_ops.fp8_linear(xs, ws)
+        p = hip_ops.act8_pack(xs)
+        assert torch.equal(y, hip_ops.fp8_matmul(p, hip_ops.fp8_weight(w.to(DEV))))
+        got = torch.autograd.grad(y, ws, dy.to(DEV))[0]
+        want, mag = _mm(dy.double().t(), held8(x)[0].t())
+        _close(got, want, (32 + 3 * M / 32 + M / 512) * U * mag, torch.float32, 'dw')
+
+
+def test_two_streams_at_once():
+    from hcmoco_amd import hip_ops
+    data = [_inputs(300, 500, 1200, torch.bfloat16, 60 + k) for k in range(2)]
+    alone = [_run(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    inputs = [[t.to(DEV) for t in d] for d in data]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for rep in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                leaves = [t.clone().requires_grad_() for t in inputs[k][:3]]
+                y = hip_ops.fp8_linear(*leaves)
+                outs[k].append([y.detach()] + list(torch.autograd.grad(y, leaves, inputs[k][3])))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for got in outs[k]:
+            assert all(torch.equal(p, q) for p, q in zip(got, alone[k]))
+
+
+def test_one_tensor_in_two_places():
+    from hcmoco_amd import hip_ops
+    x, _, _, dy = _inputs(130, 130, 130, torch.float32, 70)
+    a = x.to(DEV).requires_grad_()
+    y = hip_ops.fp8_linear(a, a)
+    y.backward(dy.to(DEV))
+    xq, wq, gq = held8(x)[0], held8(x, 128)[0], held8(dy)[0]
+    d1, m1 = _mm(gq, wq.t())
+    d2, m2 = _mm(dy.double().t(), xq.t())
+    _close(a.grad, d1 + d2, _sum_tol(130, torch.float32) * (m1 + m2) + U * (d1 + d2).abs(), torch.float32, 'dx + dw')
 
 
 def test_shapes_views_frozen_and_empty():
