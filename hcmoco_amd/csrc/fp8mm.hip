@@ -58,14 +58,14 @@ __device__ __forceinline__ void wait_loads() {
 }
 constexpr int kOutside = (int)0x80000000;       // an offset past every buffer used here (they are under 2^31 bytes)
 
-// Workgroups go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (whole columns of eight row tiles), so that
-// its L2 serves the rows they share.
+// Workgroups go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (columns of four row tiles, so
+// that 32 workgroups side by side share 4 + 8 row and column panels in its L2; eight by four: 428 against 421 us at 8192^3).
 __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in) {
   const int total = tm * tn, xcd = id & 7, k = id >> 3, base = total >> 3, rem = total & 7;
   const int t = xcd * base + min(xcd, rem) + k;
-  const int band = 8 * tn, b = t / band, in_band = t - b * band, h = min(8, tm - 8 * b);
+  const int band = 4 * tn, b = t / band, in_band = t - b * band, h = min(4, tm - 4 * b);
   in = in_band / h;
-  im = 8 * b + (in_band - in * h);
+  im = 4 * b + (in_band - in * h);
 }
 
 // thirty-two 8-bit values (the pieces g and g + 4 of a row) -> four operands of the bf16 instruction, times a power of two
@@ -120,9 +120,11 @@ __device__ __forceinline__ void out4(const Mm& P, int m, int n, v4f v) {
 // BN columns x BM rows of y a workgroup, WN x WM waves of TN x TM tiles of 16 x 16.  S LDS stages of (BN + BM) x 128 bytes in a ring;
 // one barrier a block of k, behind which the loads of the stage S - 1 blocks ahead go out between the matrix instructions (all at once
 // they block the waves' LDS reads: 480 -> 431 us at 8192^3).  Small tiles run where few workgroups do and a block of k is latency: four
-// stages.  The 256 x 256 tile is bound by these loads: 64 KB a block of k a CU take 1.4 us when
-// an XCD's workgroups, in step, all wait for the same lines from behind L2, against 1.3 us of matrix instructions and LDS reads.  So
-// each workgroup also touches, two blocks ahead, its share of the lines that the XCD's workgroups will want (431 -> 421 us).
+// stages.  The 256 x 256 tile was bound by these loads: 64 KB a block of k a CU take 1.4 us when an XCD's workgroups, in step, all wait for
+// the same lines from behind L2, against 1.25 us of matrix instructions and LDS reads.  So each workgroup also touches, two blocks
+// ahead, its share of the lines that the XCD's workgroups will want (431 -> 421 us; the loads alone then take 1.15 us a block).  What is
+// left is the two together, 1.5 us a block: the matrix pipes are busy 0.93 us of it.  Measured and not kept: four waves of 128 x 128 (spills,
+// 632 us), the barrier before the last of the eight tiles with the next block's first fragments read behind it (417 us for twice the code).
 template <int BN, int BM, int WN, int WM, int S, bool WIDE>
 __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
   constexpr int NT = WN * WM * 64, TN = BN / WN / 16, TM = BM / WM / 16;
@@ -217,9 +219,9 @@ __global__ __launch_bounds__(WN * WM * 64) void fp8_tile_kernel(const Mm P) {
     begin(kb + S - 1);
     const int next = buf == 0 ? S - 1 : buf - 1;
     if constexpr (TOUCH) {
-      // of the eight row tiles and four column tiles that run side by side on an XCD: an eighth of this tile's W rows, a quarter of its X rows
+      // of the four row tiles and eight column tiles that run side by side on an XCD: a quarter of this tile's W rows, an eighth of its X rows
       if (wave < 2 && kb + 2 < k_to) {
-        const int r = wave ? (im & 7) * (BN / 8) + (lane & (BN / 8 - 1)) : (in & 3) * (BM / 4) + (lane & (BM / 4 - 1));
+        const int r = wave ? (im & 3) * (BN / 4) + (lane & (BN / 4 - 1)) : (in & 7) * (BM / 8) + (lane & (BM / 8 - 1));
         if (wave) load_lds<4>(make_rsrc(wbase, wbytes), lds_addr(touched + 64), r * (int)P.ldw + (kb + 2) * 128);
         else load_lds<4>(make_rsrc(xbase, xbytes), lds_addr(touched), r * (int)P.ldx + (kb + 2) * 128);
       }
