@@ -144,7 +144,7 @@ SIGNATURES = {
     'hcm_fp8_matmul': (_i, [_p, _i64] * 4 + [_p] + [_i] * 4 + [_p, _i, _p, _sz, _p]),
     'hcm_fp8_rows_supported': (_i, [_i64, _i]),
     'hcm_fp8_rows': (_i, [_p, _i, _i64] + [_p, _i64] * 2 + [_p] + [_i] * 4 + [_p] * 4),
-    'hcm_fp8_wgrad_workspace_bytes': (_sz, [_i64, _i, _i, _i]),
+    'hcm_fp8_wgrad_workspace_bytes': (_sz, [_i64, _i, _i, _i, _i]),
     'hcm_fp8_wgrad': (_i, [_p, _i64, _p, _i64, _p, _i, _i64, _i, _i, _p, _i, _p, _i, _p, _sz, _p]),
     'hcm_layer_norm_forward': (_i, [_p, _i, _i64, _i, _i64, _p, _i, _p, _i, _f, _p, _p, _p, _p, _i64, _p, _i64, _p]),
     'hcm_layer_norm_backward_workspace_bytes': (_sz, [_i64, _i]),

@@ -783,20 +783,22 @@ int hcm_fp8_rows(const void* x, int dtype, int64_t ldx, const uint8_t* w, int64_
 // partial sums of dW and db, a multiple of four floats apart
 static int64_t wgrad_stride(int N, int K) { return ((int64_t)N * K + N + 3) / 4 * 4; }
 
-size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K, int dy_dtype) {
+size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K, int dy_dtype, int with_dw) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (!with_dw) K = 1;
   const WgPlan p = wgrad_plan(M, N, K, dy_dtype);
   return p.split > 1 ? (size_t)p.split * wgrad_stride(N, K) * sizeof(float) : 0;
 }
 
 int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldsx, const void* dy, int dy_dtype, int64_t M, int N, int K, void* dw,
                   int dw_dtype, void* db, int db_dtype, void* workspace, size_t workspace_bytes, hcm_stream_t stream) {
-  if (!x || !x_scale || !dy || (!dw && !db) || M <= 0 || M >= (1ll << 31) || N <= 0 || K <= 0 || K > (1 << 22) || N > (1 << 22) ||
+  if ((dw && (!x || !x_scale)) || !dy || (!dw && !db) || M <= 0 || M >= (1ll << 31) || N <= 0 || K <= 0 || K > (1 << 22) || N > (1 << 22) ||
       ldx != hcm_act8_pitch(K) || ldsx != hcm_act8_scale_pitch(K) || dy_dtype < 0 || dy_dtype > 2 || dw_dtype < 0 || dw_dtype > 2 || db_dtype < 0 ||
       db_dtype > 2 || ((uintptr_t)x & 15) || ((uintptr_t)dy & 15))
     return (int)hipErrorInvalidValue;
+  if (!dw) x = x_scale = nullptr, ldx = ldsx = 0, K = 1;       // the sums of dy's columns alone: one column of tiles, an X of no bytes
   const WgPlan p = wgrad_plan(M, N, K, dy_dtype);
-  if (p.split > 1 && (!workspace || workspace_bytes < hcm_fp8_wgrad_workspace_bytes(M, N, K, dy_dtype))) return (int)hipErrorInvalidValue;
+  if (p.split > 1 && (!workspace || workspace_bytes < hcm_fp8_wgrad_workspace_bytes(M, N, K, dy_dtype, dw != nullptr))) return (int)hipErrorInvalidValue;
   const int64_t tiles = (int64_t)((K + p.tk - 1) / p.tk) * ((N + p.tn - 1) / p.tn), steps = (M + kWgRows - 1) / kWgRows;
   if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
   const Wg G = {x,  x_scale, ldx, ldsx, dy, M, N, K, (steps + p.split - 1) / p.split * kWgRows, p.split > 1 ? (float*)workspace : nullptr, wgrad_stride(N, K),

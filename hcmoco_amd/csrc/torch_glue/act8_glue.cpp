@@ -233,16 +233,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> fp8_weight(const Tensor& weight) {
   return {q, scale, qt, scale_t};
 }
 
-// y [M, N] = X W^T + bias, everything checked by the caller
-Tensor product(const Packed& x, int64_t M, const Tensor& wq, const Tensor& ws, int64_t N, int64_t K, const Tensor& bias, at::IntArrayRef shape,
-               at::ScalarType dtype) {
-  Tensor y = at::empty(shape, x.q.options().dtype(dtype));
+// y [M, N] = X W^T + bias on buffers of the pitches of K, everything checked by the caller; `like`: the device
+Tensor product(const uint8_t* xq, const uint8_t* xs, int64_t M, const uint8_t* wq, const uint8_t* ws, int64_t N, int64_t K, const Tensor& bias,
+               at::IntArrayRef shape, at::ScalarType dtype, const Tensor& like) {
+  Tensor y = at::empty(shape, like.options().dtype(dtype));
   if (M) {
     const int dt = dt_of(dtype, "fp8_matmul");
     const size_t n = hcm_fp8_matmul_workspace_bytes((int)M, (int)N, (int)K, dt);
-    const Tensor work = workspace(n, x.q);
-    check_rc(hcm_fp8_matmul(bytes(x.q), x.q.size(1), bytes(x.scale), x.scale.size(1), bytes(wq), wq.size(1), bytes(ws), ws.size(1), ptr(bias),
-                            dt_of(bias, "fp8_matmul"), (int)M, (int)N, (int)K, y.data_ptr(), dt, ptr(work), n, stream_of(x.q)),
+    const Tensor work = workspace(n, like);
+    const int64_t pitch = hcm_act8_pitch(K), sp = hcm_act8_scale_pitch(K);
+    check_rc(hcm_fp8_matmul(xq, pitch, xs, sp, wq, pitch, ws, sp, ptr(bias), dt_of(bias, "fp8_matmul"), (int)M, (int)N, (int)K, y.data_ptr(), dt, ptr(work),
+                            n, stream_of(like)),
              "hcm_fp8_matmul");
   }
   return y;
@@ -273,45 +274,79 @@ Tensor fp8_matmul(const Tensor& q, const Tensor& scale, at::IntArrayRef shape, c
   const Tensor b = value(bias);
   check_vector(b, q, N, "fp8_matmul", "bias");
   const c10::DeviceGuard guard(q.device());
-  return product({q, scale}, M, wq, ws, N, K, b, with_last(shape, N), dtype);
+  return product(bytes(q), bytes(scale), M, bytes(wq), bytes(ws), N, K, b, with_last(shape, N), dtype, q);
 }
 
-// Q(x) W^T + bias for x as it comes; `packed`: Q(x) is wanted too
-Tensor linear_forward(const Rows& r, const Tensor& wq, const Tensor& ws, int64_t N, const Tensor& bias, at::IntArrayRef shape, Packed* packed) {
-  if (!hcm_fp8_rows_supported(r.rows, r.cols)) {
-    Packed a = pack_raw(r, "fp8_linear");
-    Tensor y = product(a, r.rows, wq, ws, N, r.cols, bias, shape, r.t.scalar_type());
-    if (packed) *packed = a;
-    return y;
+// Where the parts of a laid-out weight lie: in the four tensors of an Fp8Weight, or one behind the other in one buffer (a training step
+// lays its weight out anew on every call, and four allocations would cost more host time than the launch).
+struct Weight8 {
+  Tensor first, second;              // what the backward pass keeps: the buffer; or qt and scale_t
+  const uint8_t *q, *scale, *qt, *scale_t;
+};
+Weight8 weight_in(const Tensor& buffer, int64_t N, int64_t K) {
+  Weight8 w;
+  w.first = buffer;
+  w.q = bytes(buffer);
+  w.qt = w.q + N * hcm_act8_pitch(K);
+  w.scale = w.qt + K * hcm_act8_pitch(N);
+  w.scale_t = w.scale + (N + 127) / 128 * hcm_act8_scale_pitch(K);
+  return w;
+}
+Weight8 lay_out(const Tensor& weight) {
+  const Rows r = rows_of(weight, "fp8_linear");
+  const int64_t N = r.rows, K = r.cols;
+  TORCH_CHECK_VALUE(N > 0 && N <= kMaxSide && K <= kMaxSide, "fp8_linear: expected a weight [N, K] with both in 1..2^22, got ", weight.sizes());
+  const int64_t size = N * hcm_act8_pitch(K) + K * hcm_act8_pitch(N) + (N + 127) / 128 * hcm_act8_scale_pitch(K) + (K + 127) / 128 * hcm_act8_scale_pitch(N);
+  Weight8 w = weight_in(workspace(size, weight), N, K);
+  check_rc(hcm_fp8_weight_pack(r.t.data_ptr(), dt_of(weight, "fp8_linear"), (int)N, (int)K, r.ld, (uint8_t*)w.q, hcm_act8_pitch(K), (uint8_t*)w.scale,
+                               hcm_act8_scale_pitch(K), (uint8_t*)w.qt, hcm_act8_pitch(N), (uint8_t*)w.scale_t, hcm_act8_scale_pitch(N), stream_of(weight)),
+           "hcm_fp8_weight_pack");
+  return w;
+}
+
+// Q(x) W^T + bias for x as it comes.  `packed`: Q(x) is wanted too, its scales behind its values in one buffer.
+Tensor linear_forward(const Rows& r, const uint8_t* wq, const uint8_t* ws, int64_t N, const Tensor& bias, at::IntArrayRef shape, Tensor* packed) {
+  const bool few = hcm_fp8_rows_supported(r.rows, r.cols);
+  const int64_t pitch = hcm_act8_pitch(r.cols), sp = hcm_act8_scale_pitch(r.cols);
+  Tensor buffer;
+  uint8_t *q = nullptr, *scale = nullptr;
+  if (packed || !few) {
+    buffer = at::empty({r.rows * (pitch + sp)}, r.t.options().dtype(at::kByte));
+    q = bytes(buffer);
+    scale = q + r.rows * pitch;
   }
-  Packed a;
-  if (packed) a = *packed = packed_buffers(r.rows, r.cols, r.t);
+  if (packed) *packed = buffer;
+  const int dt = dt_of(r.t, "fp8_linear");
+  if (!few) {
+    if (r.rows) check_rc(hcm_act8_pack(r.t.data_ptr(), dt, r.rows, r.cols, r.ld, q, pitch, scale, sp, stream_of(r.t)), "hcm_act8_pack");
+    return product(q, scale, r.rows, wq, ws, N, r.cols, bias, shape, r.t.scalar_type(), r.t);
+  }
   Tensor y = at::empty(shape, r.t.options());
-  check_rc(hcm_fp8_rows(r.t.data_ptr(), dt_of(r.t, "fp8_linear"), r.ld, bytes(wq), wq.size(1), bytes(ws), ws.size(1), ptr(bias), dt_of(bias, "fp8_linear"),
-                        (int)r.rows, (int)N, r.cols, y.data_ptr(), bytes(a.q), bytes(a.scale), stream_of(r.t)),
+  check_rc(hcm_fp8_rows(r.t.data_ptr(), dt, r.ld, wq, pitch, ws, sp, ptr(bias), dt_of(bias, "fp8_linear"), (int)r.rows, (int)N, r.cols, y.data_ptr(), q, scale,
+                        stream_of(r.t)),
            "hcm_fp8_rows");
   return y;
 }
 
 struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Tensor& wq, const Tensor& ws,
-                        const Tensor& wqt, const Tensor& wst, int64_t N) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight, const OptTensor& bias, const Weight8& W, int64_t N) {
     const Tensor w = value(weight), b = value(bias);
     const Rows r = rows_of(x, "fp8_linear");
-    Packed a;
-    Tensor y = linear_forward(r, wq, ws, N, b, with_last(x.sizes(), N), &a);
+    const bool nx = wants_grad(x), nw = wants_grad(w);
+    Tensor packed;
+    Tensor y = linear_forward(r, W.q, W.scale, N, b, with_last(x.sizes(), N), nw ? &packed : nullptr);
     // x itself is not kept: the 8-bit operand of this product is the checkpoint that the weight's gradient reads
-    ctx->save_for_backward({a.q, a.scale, wqt, wst});
-    ctx->saved_data["m"] = std::vector<int64_t>{r.rows, N, r.cols, wants_grad(x), wants_grad(w), wants_grad(b),
-                                                w.defined() ? (int64_t)w.scalar_type() : 0, b.defined() ? (int64_t)b.scalar_type() : 0};
-    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->save_for_backward({packed, nx ? W.first : Tensor(), nx ? W.second : Tensor()});
+    std::vector<int64_t> m{r.rows, N, r.cols, nx, nw, wants_grad(b), nw ? (int64_t)w.scalar_type() : 0, b.defined() ? (int64_t)b.scalar_type() : 0};
+    m.insert(m.end(), x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["m"] = std::move(m);
     return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto m = ctx->saved_data["m"].toIntVector();
-    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const at::IntArrayRef shape(m.data() + 8, m.size() - 8);
     const int64_t M = m[0], N = m[1], K = m[2];
     const bool nx = m[3], nw = m[4], nb = m[5];
     Tensor dx, dw, db;
@@ -320,21 +355,28 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       Tensor dy = grads[0].contiguous();
       if ((uintptr_t)dy.data_ptr() & 15) dy = dy.clone();        // a view that begins anywhere: hcm_fp8_wgrad reads 16-byte pieces
       const c10::DeviceGuard guard(dy.device());
+      if (nx) {
+        Weight8 W;
+        if (saved[2].defined()) W.qt = bytes(saved[1]), W.scale_t = bytes(saved[2]);
+        else W = weight_in(saved[1], N, K);
+        dx = linear_forward({dy, M, N, (int)N}, W.qt, W.scale_t, K, Tensor(), shape, nullptr);
+      }
       if (nw) dw = at::empty({N, K}, dy.options().dtype((at::ScalarType)m[6]));
       if (nb) db = at::empty({N}, dy.options().dtype((at::ScalarType)m[7]));
-      if (nx) dx = linear_forward({dy, M, N, (int)N}, saved[2], saved[3], K, Tensor(), shape, nullptr);
       if ((nw || nb) && M) {
-        const size_t n = hcm_fp8_wgrad_workspace_bytes(M, (int)N, (int)K, dt_of(dy, "fp8_linear"));
+        const int dt = dt_of(dy, "fp8_linear");
+        const size_t n = hcm_fp8_wgrad_workspace_bytes(M, (int)N, (int)K, dt, nw);
         const Tensor work = workspace(n, dy);
-        check_rc(hcm_fp8_wgrad(bytes(saved[0]), saved[0].size(1), bytes(saved[1]), saved[1].size(1), dy.data_ptr(), dt_of(dy, "fp8_linear"), M, (int)N,
-                               (int)K, ptr(dw), dt_of(dw, "fp8_linear"), ptr(db), dt_of(db, "fp8_linear"), ptr(work), n, stream_of(dy)),
+        const uint8_t* q = nw ? bytes(saved[0]) : nullptr;
+        check_rc(hcm_fp8_wgrad(q, hcm_act8_pitch(K), nw ? q + M * hcm_act8_pitch(K) : nullptr, hcm_act8_scale_pitch(K), dy.data_ptr(), dt, M, (int)N, (int)K,
+                               ptr(dw), dt_of(dw, "fp8_linear"), ptr(db), dt_of(db, "fp8_linear"), ptr(work), n, stream_of(dy)),
                  "hcm_fp8_wgrad");
       } else {
         if (nw) dw.zero_();
         if (nb) db.zero_();
       }
     }
-    return once({dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    return once({dx, dw, db, Tensor(), Tensor()});
   }
 };
 
@@ -345,7 +387,6 @@ Tensor fp8_linear(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "fp8_linear: the last axis must have at least one element");
   const int64_t K = x.size(-1);
   const Tensor w = value(weight), b = value(bias);
-  Tensor wq, ws, wqt, wst;
   if (w.defined()) {
     check_float(w, x, "fp8_linear");
     w_shape = w.sizes();
@@ -354,20 +395,22 @@ Tensor fp8_linear(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   check_width(K, w_shape[1], "fp8_linear");
   const int64_t N = w_shape[0];
   check_vector(b, x, N, "fp8_linear", "bias");
+  TORCH_CHECK_VALUE(x.numel() / K <= INT32_MAX - 512, "fp8_linear: too many rows");
   const c10::DeviceGuard guard(x.device());
+  Weight8 W;
   if (w.defined()) {
-    std::tie(wq, ws, wqt, wst) = fp8_weight(w);
+    at::AutoGradMode off(false);
+    W = lay_out(w);
   } else {
-    wq = value(wq_), ws = value(ws_), wqt = value(wqt_), wst = value(wst_);
+    const Tensor wq = value(wq_), ws = value(ws_), wqt = value(wqt_), wst = value(wst_);
     TORCH_CHECK_VALUE(wq.defined() && ws.defined() && wqt.defined() && wst.defined(), "fp8_linear: no weight");
     check_weight(wq, ws, N, K, x, "fp8_linear");
     check_weight(wqt, wst, K, N, x, "fp8_linear");
+    W = {wqt, wst, bytes(wq), bytes(ws), bytes(wqt), bytes(wst)};
   }
-  TORCH_CHECK_VALUE(x.numel() / K <= INT32_MAX - 512, "fp8_linear: too many rows");
-  if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) {
-    return linear_forward(rows_of(x, "fp8_linear"), wq, ws, N, b, with_last(x.sizes(), N), nullptr);
-  }
-  return Fp8Linear::apply(x, weight, bias, wq, ws, wqt, wst, N);
+  if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b)))
+    return linear_forward(rows_of(x, "fp8_linear"), W.q, W.scale, N, b, with_last(x.sizes(), N), nullptr);
+  return Fp8Linear::apply(x, weight, bias, W, N);
 }
 
 }  // namespace

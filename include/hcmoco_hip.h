@@ -759,8 +759,9 @@ int hcm_fp8_rows_supported(int64_t M, int K);
 int hcm_fp8_rows(const void* x, int dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const uint8_t* w_scale, int64_t ldsw,
                  const void* bias, int bias_dtype, int M, int N, int K, void* y, uint8_t* q, uint8_t* q_scale, hcm_stream_t stream);
 /* dw [N, K] = dy^T X and db [N] = sum of dy's rows, for dy [M, N] and X [M, K] the 8-bit checkpoint: products of exact values, fp32
- * sums, fixed order.  dy contiguous, 16-byte aligned.  dw or db: NULL = not wanted. */
-size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K, int dy_dtype);
+ * sums, fixed order.  dy contiguous, 16-byte aligned.  dw or db: NULL = not wanted; without dw
+ * (with_dw 0) x may be NULL. */
+size_t hcm_fp8_wgrad_workspace_bytes(int64_t M, int N, int K, int dy_dtype, int with_dw);
 int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldsx, const void* dy, int dy_dtype, int64_t M, int N,
                   int K, void* dw, int dw_dtype, void* db, int db_dtype, void* workspace, size_t workspace_bytes, hcm_stream_t stream);
 

@@ -81,8 +81,8 @@ def test_products_refuse():
         a = {**good, **bad}
         assert L.hcm_fp8_rows(*[a[k] for k in good], Z) != 0, bad
     assert [L.hcm_fp8_rows_supported(*a) for a in ((1, 32768), (1, 32769), (32, 1024), (32, 1025), (33, 1), (0, 1))] == [1, 0, 1, 0, 0, 0]
-    need = L.hcm_fp8_wgrad_workspace_bytes(4000, 200, 270, 0)
-    assert need > 0 and L.hcm_fp8_wgrad_workspace_bytes(8192, 4096, 4096, 1) == 0
+    need = L.hcm_fp8_wgrad_workspace_bytes(4000, 200, 270, 0, 1)
+    assert need > 0 and L.hcm_fp8_wgrad_workspace_bytes(8192, 4096, 4096, 1, 1) == 0
     good = dict(x=P, ldx=272, sx=P, ldsx=4, dy=P, dd=0, M=4000, N=200, K=270, dw=P, wd=0, db=P, bd=0, ws=P, n=need)
     for bad in (dict(x=Z), dict(ldx=270), dict(sx=Z), dict(ldsx=2), dict(dy=Z), dict(dd=3), dict(M=0), dict(M=2 ** 31), dict(N=0), dict(K=0),
                 dict(N=2 ** 22 + 1), dict(dw=Z, db=Z), dict(wd=9), dict(bd=-1), dict(ws=Z), dict(n=need - 1), dict(x=C.c_void_p(4104)), dict(dy=C.c_void_p(4104))):

@@ -258,6 +258,18 @@ def test_shapes_views_frozen_and_empty():
     assert kept.nbytes() < 3 * w.numel()
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,N', [(5, 3), (40, 130), (3000, 257), (20000, 1000)])
+def test_bias_alone(M, N, dtype):
+    """A frozen weight: nothing of x is kept, the bias's gradient is the sum of dy's rows."""
+    from hcmoco_amd import hip_ops
+    x, w, b, dy = _inputs(M, N, 70, dtype, M)
+    bias = b.to(DEV).requires_grad_()
+    y = hip_ops.fp8_linear(x.to(DEV), hip_ops.fp8_weight(w.to(DEV)), bias)
+    got, = torch.autograd.grad(y, bias, dy.to(DEV))
+    _close(got, dy.double().sum(0), (32 + 3 * M / 32 + M / 512) * U * dy.double().abs().sum(0), torch.float32, 'db')
+
+
 def test_a_block_of_layers():
     """layer norm -> linear -> layer norm (8-bit checkpoint) -> linear, forward and backward in one graph: every stage against its
     formulas on the tensors that it was really given."""
