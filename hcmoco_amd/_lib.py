@@ -140,7 +140,7 @@ SIGNATURES = {
     'hcm_act8_pack': (_i, [_p, _i, _i64, _i, _i64, _p, _i64, _p, _i64, _p]),
     'hcm_act8_unpack': (_i, [_p, _i64, _p, _i64, _i64, _i, _p, _i, _p]),
     'hcm_fp8_weight_pack': (_i, [_p, _i, _i, _i, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p]),
-    'hcm_fp8_matmul_workspace_bytes': (_sz, [_i] * 4),
+    'hcm_fp8_matmul_workspace_bytes': (_sz, [_i] * 3),
     'hcm_fp8_matmul': (_i, [_p, _i64] * 4 + [_p] + [_i] * 4 + [_p, _i, _p, _sz, _p]),
     'hcm_fp8_rows_supported': (_i, [_i64, _i]),
     'hcm_fp8_rows': (_i, [_p, _i, _i64] + [_p, _i64] * 2 + [_p] + [_i] * 4 + [_p] * 4),

@@ -12,7 +12,7 @@
 // 16x16x32; the sums of groups are full fp32): 2e-5 .. 7e-5 of the result's norm on random data.  That is under the rounding of
 // a 16-bit y (2^-9, 2^-12), and it is over that of an fp32 one, so y in fp32 takes the WIDE form: the 8-bit values are widened to bf16
 // on their way from LDS -- exact, the scales included, by v_cvt_scalef32_pk_bf16_fp8 -- and multiplied by v_mfma_f32_16x16x32_bf16,
-// whose sums are fp32 (1e-8 .. 3e-7 on the same data), at half the rate.
+// whose sums are fp32 (1e-8 .. 3e-7 on the same data), at half the rate (8192 x 4096 x 4096: 1.33 PFLOP/s; 2.4 in 8 bits).
 #include <cmath>
 #include "act8.h"
 #include "../../include/hcmoco_hip.h"
@@ -709,13 +709,15 @@ void tile_launch(bool wide, const dim3& grid, const Mm& P, hipStream_t st) {
 
 struct Plan { int tile, split; };      // tile: columns = rows of a workgroup's tile
 
-// `wide`: the bf16 operands of a 256 x 256 tile do not fit the registers
-Plan plan(int M, int N, int kblocks, bool wide) {
+// The largest tile that leaves enough workgroups and is not padded away; a contraction is split where they do not fill the CUs.
+//   256: from 128 tiles up (3000 x 3000 x 4000 in bf16, 144 tiles on 256 CUs: 53 us, 128-wide tiles 71; 2500 x 2500 x 5000, 100 tiles: 65
+//   against 50), unsplit, unless it computes over 1.3 times what 128-wide tiles would (131072 x 128 x 270 in bf16: 26 against 21 us)
+Plan plan(int M, int N, int kblocks) {
   auto tiles = [&](int t) { return (int64_t)((M + t - 1) / t) * ((N + t - 1) / t); };
-  const int tile = tiles(256) >= 192 && !wide ? 256 : tiles(128) >= 192 ? 128 : 64;
+  const int tile = tiles(256) >= 128 && tiles(256) * 40 <= tiles(128) * 13 ? 256 : tiles(128) >= 192 ? 128 : 64;
   int split = 1;
   const int64_t have = tiles(tile);
-  if (have < 256) split = (int)((512 + have - 1) / have);
+  if (have < 256 && tile < 256) split = (int)((512 + have - 1) / have);
   if (split > kblocks / 4) split = kblocks / 4;
   if (split > 16) split = 16;
   if (split < 1) split = 1;
@@ -726,9 +728,9 @@ Plan plan(int M, int N, int kblocks, bool wide) {
 
 extern "C" {
 
-size_t hcm_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype) {
+size_t hcm_fp8_matmul_workspace_bytes(int M, int N, int K) {
   if (M <= kFewRows || N <= 0 || K <= 0) return 0;
-  const Plan p = plan(M, N, (K + 127) / 128, out_dtype == kF32);
+  const Plan p = plan(M, N, (K + 127) / 128);
   return p.split > 1 ? (size_t)p.split * M * N * sizeof(float) : 0;
 }
 
@@ -744,17 +746,19 @@ int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   hipStream_t st = (hipStream_t)stream;
   if (M <= kFewRows)
     return wide ? few<uint8_t, true>(P, nullptr, 0, K, nullptr, nullptr, st) : few<uint8_t, false>(P, nullptr, 0, K, nullptr, nullptr, st);
-  const Plan p = plan(M, N, P.kblocks, wide);
-  if (workspace_bytes < hcm_fp8_matmul_workspace_bytes(M, N, K, out_dtype) || (p.split > 1 && !workspace)) return (int)hipErrorInvalidValue;
+  const Plan p = plan(M, N, P.kblocks);
+  if (workspace_bytes < hcm_fp8_matmul_workspace_bytes(M, N, K) || (p.split > 1 && !workspace)) return (int)hipErrorInvalidValue;
   P.split = p.split;
   if (p.split > 1) P.part = (float*)workspace;
   const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((N + p.tile - 1) / p.tile);
   if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
   const dim3 grid((uint32_t)tiles, 1, p.split);
-  // Four stages keep a long contraction fed where few workgroups run (500 x 4096 x 4096: 21.8 -> 17.4 us); a short one has no use for
-  // them, and two stages leave room for a second workgroup on the CU (131072 x 128 x 270 in fp32: 41.7 -> 30.6 us).
-  const bool deep = P.kblocks > 4;
-  if (p.tile == 256) fp8_tile_kernel<256, 256, 2, 4, 2, false><<<grid, 512, 0, st>>>(P);
+  // Four stages keep a long contraction fed where each CU has no more workgroups than fit beside each other with them (one of 128-wide
+  // tiles, two of 64: 500 x 4096 x 4096 in bf16 21.8 -> 17.4 us); where it has more, two stages and twice the workgroups at once are
+  // faster (1000 x 5000 x 1000 in bf16: 20.6 -> 14.1 us; 131072 x 128 x 270 in fp32: 41.7 -> 30.6 us).
+  const bool deep = P.kblocks > 4 && tiles * p.split <= (p.tile == 128 ? 256 : 512);
+  if (p.tile == 256 && wide) fp8_tile_kernel<256, 256, 2, 4, 2, true><<<grid, 512, 0, st>>>(P);
+  else if (p.tile == 256) fp8_tile_kernel<256, 256, 2, 4, 2, false><<<grid, 512, 0, st>>>(P);
   else if (p.tile == 128) deep ? tile_launch<128, 4>(wide, grid, P, st) : tile_launch<128, 2>(wide, grid, P, st);
   else deep ? tile_launch<64, 4>(wide, grid, P, st) : tile_launch<64, 2>(wide, grid, P, st);
   HCM_CHECK_LAUNCH();

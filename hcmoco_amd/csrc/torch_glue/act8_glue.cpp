@@ -239,7 +239,7 @@ Tensor product(const uint8_t* xq, const uint8_t* xs, int64_t M, const uint8_t* w
   Tensor y = at::empty(shape, like.options().dtype(dtype));
   if (M) {
     const int dt = dt_of(dtype, "fp8_matmul");
-    const size_t n = hcm_fp8_matmul_workspace_bytes((int)M, (int)N, (int)K, dt);
+    const size_t n = hcm_fp8_matmul_workspace_bytes((int)M, (int)N, (int)K);
     const Tensor work = workspace(n, like);
     const int64_t pitch = hcm_act8_pitch(K), sp = hcm_act8_scale_pitch(K);
     check_rc(hcm_fp8_matmul(xq, pitch, xs, sp, wq, pitch, ws, sp, ptr(bias), dt_of(bias, "fp8_matmul"), (int)M, (int)N, (int)K, y.data_ptr(), dt, ptr(work),

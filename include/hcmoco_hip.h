@@ -749,7 +749,7 @@ int hcm_fp8_weight_pack(const void* w, int dtype, int rows, int cols, int64_t ld
  * A workspace of hcm_fp8_matmul_workspace_bytes (0: NULL is fine)
  * holds partial sums where the contraction
  * is split; they are joined in a fixed order.  N, K <= 2^22. */
-size_t hcm_fp8_matmul_workspace_bytes(int M, int N, int K, int out_dtype);
+size_t hcm_fp8_matmul_workspace_bytes(int M, int N, int K);
 int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t ldsx, const uint8_t* w, int64_t ldw,
                    const uint8_t* w_scale, int64_t ldsw, const void* bias, int bias_dtype, int M, int N, int K, void* y, int out_dtype,
                    void* workspace, size_t workspace_bytes, hcm_stream_t stream);

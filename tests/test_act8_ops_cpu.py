@@ -69,8 +69,8 @@ def test_products_refuse():
                 dict(x=C.c_void_p(4104)), dict(w=C.c_void_p(4104)), dict(sx=C.c_void_p(4097)), dict(sw=C.c_void_p(4098))):
         a = {**good, **bad}
         assert L.hcm_fp8_matmul(*[a[k] for k in good], Z) != 0, bad
-    need = L.hcm_fp8_matmul_workspace_bytes(64, 128, 4096, 0)
-    assert need > 0 and L.hcm_fp8_matmul_workspace_bytes(8192, 8192, 8192, 1) == 0 and L.hcm_fp8_matmul_workspace_bytes(0, 1, 1, 0) == 0
+    need = L.hcm_fp8_matmul_workspace_bytes(64, 128, 4096)
+    assert need > 0 and L.hcm_fp8_matmul_workspace_bytes(8192, 8192, 8192) == 0 and L.hcm_fp8_matmul_workspace_bytes(0, 1, 1) == 0
     a = {**good, **dict(ldx=4096, ldw=4096, ldsx=32, ldsw=32, M=64, N=128, K=4096)}
     for bad in (dict(n=need - 1), dict(ws=Z)):
         assert L.hcm_fp8_matmul(*[{**a, **bad}[k] for k in good], Z) != 0, bad

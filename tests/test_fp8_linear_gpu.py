@@ -84,8 +84,9 @@ def test_training_step(M, N, K, dtype):
 @pytest.mark.parametrize('M,N,K', [(3500, 3600, 300), (1800, 1900, 200), (3000, 100, 1300), (40, 4000, 700), (1000, 2040, 2049), (333, 2100, 2300),
                                    (4200, 264, 1900)])
 def test_every_tile_and_split(M, N, K):
-    x, w, b, dy = _inputs(M, N, K, torch.bfloat16, 7)
-    _check_step(x, w, None, dy, _run(x, w, None, dy))
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w, b, dy = _inputs(M, N, K, dtype, 7)
+        _check_step(x, w, None, dy, _run(x, w, None, dy))
 
 
 def test_gradient_that_begins_anywhere():
