@@ -480,10 +480,10 @@ __device__ __forceinline__ void pieces(const float (&v)[8], v8bf (&out)[P]) {
 // DIRECT, dy (bf16, rows of 16-byte pieces) goes from memory to LDS by itself, and only X, which is widened on the way, through registers.
 template <typename T, int P, int TK, int TN, int ROWS, int WK, int WN, bool DIRECT>
 __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
-  constexpr int FA = TK / WK / 16, FB = TN / WN / 16, AHEAD = DIRECT || TK == 384 ? 1 : 2;
-  constexpr int RG = ROWS / 32, CX = TK / 128 * RG, CD = DIRECT ? 4 : RG;      // pieces a thread moves: eight values, sixteen threads a row of 128
+  constexpr int FA = TK / WK / 16, FB = TN / WN / 16, AHEAD = DIRECT || TK == 384 || TN == 256 ? 1 : 2;
+  constexpr int RG = ROWS / 32, CX = TK / 128 * RG, CD = DIRECT ? 4 : TN / 128 * RG;      // pieces a thread moves: eight values, sixteen threads a row of 128
   constexpr int XBYTES = ROWS * TK * 2, DBYTES = ROWS * TN * 2;
-  static_assert(WK * WN == 8 && TK % 128 == 0 && kWgRows % ROWS == 0 && (DIRECT ? P == 1 && TN == 256 && ROWS == 64 && FB == CD : TN == 128), "shape");
+  static_assert(WK * WN == 8 && TK % 128 == 0 && kWgRows % ROWS == 0 && (DIRECT ? P == 1 && TN == 256 && ROWS == 64 && FB == CD : TN % 128 == 0), "shape");
   // X as bf16 [ROWS][TK], then the P pieces of dy [ROWS][TN]; 16-byte piece c of row r in slot c ^ swz(r): the four rows that
   // sixteen lanes of a transpose read touch lie in different banks
   __shared__ __attribute__((aligned(16))) uint8_t stage[2][XBYTES + P * DBYTES];
@@ -498,8 +498,8 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
   const int x_off = tr * (int)G.ldq + k0 + tc * 8, x_left = (int)G.ldq - k0 - tc * 8, s_off = tr * (int)G.lds + k0 / 128;
   struct Set { v2i xq[CX]; int xs[CX]; typename Vec8<T>::type d[DIRECT ? 1 : CD]; };
   Set set[AHEAD];
-  float cs[DIRECT ? 1 : 8] = {};       // of the columns tc * 8 .. + 7 of dy, this thread's rows
-  auto d_at = [&](int64_t m, int j) { return (m + tr + j * 32) * G.N + n0 + tc * 8; };
+  float cs[DIRECT ? 1 : TN / 128][8] = {};       // of the columns tc * 8 .. + 7 of each 128 of dy, this thread's rows
+  auto d_at = [&](int64_t m, int j) { return (m + tr + j % RG * 32) * G.N + n0 + j / RG * 128 + tc * 8; };
   // The stage that begins at m.  Rows of X past the split's end read as zero; of dy they are made zero in put().
   auto fetch = [&](Set& S, int64_t m) {
     const int rows = (int)max((int64_t)0, min(m_to - m, (int64_t)ROWS));
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
     }
 #pragma unroll
     for (int j = 0; j < (DIRECT ? 0 : CD); ++j) {
-      const int row = tr + j * 32, at = XBYTES + row * TN * 2 + ((tc ^ swz(row)) << 4);
+      const int row = tr + j % RG * 32, at = XBYTES + row * TN * 2 + (((j / RG * 16 + tc) ^ swz(row)) << 4);
       // columns past N are whatever lies there: their sums are not stored
       const int64_t from = d_at(m, j);
       if (m + row >= m_to) {
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
       }
       if (!DIRECT && ik == 0) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) cs[DIRECT ? 0 : q] += (float)S.d[j][q];
+        for (int q = 0; q < 8; ++q) cs[DIRECT ? 0 : j / RG][q] += (float)S.d[j][q];
       }
       if constexpr (P == 1) {
         *(v8bf*)(stage[buf] + at) = __builtin_bit_cast(v8bf, S.d[j]);
@@ -655,33 +655,40 @@ __global__ __launch_bounds__(512) void fp8_wgrad_kernel(const Wg G) {
     }
   }
   if (!DIRECT && ik == 0) {
-    float* red = (float*)stage;        // [8][128]; the last step ended with a barrier
+    float* red = (float*)stage;        // [8][TN]; the last step ended with a barrier
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      float v = cs[DIRECT ? 0 : q];
-      v += __shfl_xor(v, 16, 64);
-      v += __shfl_xor(v, 32, 64);
-      if (lane < 16) red[wave * 128 + tc * 8 + q] = v;
-    }
+    for (int c = 0; c < (DIRECT ? 1 : TN / 128); ++c)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float v = cs[c][q];
+        v += __shfl_xor(v, 16, 64);
+        v += __shfl_xor(v, 32, 64);
+        if (lane < 16) red[wave * TN + c * 128 + tc * 8 + q] = v;
+      }
     __syncthreads();
-    if (t < 128 && n0 + t < G.N) {
+    if (t < TN && n0 + t < G.N) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) v += red[w * 128 + t];
+      for (int w = 0; w < 8; ++w) v += red[w * TN + t];
       if (part) part[(int64_t)G.N * G.K + n0 + t] = v;
       else if (G.db) store_dt(G.db, G.db_dt, n0 + t, v);
     }
   }
 }
 
-// The tile of dW: 256 x 256 where that leaves enough workgroups and dy can go to LDS directly (bf16, rows of 16-byte pieces).  Else 128
-// columns n, and of 384, 256 or 128 columns k those that pad K least (K = 270: 384; 131072 rows of fp32, N = 128).
+// dy that goes to LDS directly: bf16, rows of 16-byte pieces
+static bool wgrad_direct(int N, int dy_dt) { return dy_dt == kBF16 && N % 8 == 0; }
+
+// The tile of dW: 256 x 256 where that leaves enough workgroups, and where dy goes through registers, stages of half the rows, enough rows
+// (fp16 dy, 128 wide against 256: 8192 x 4096 x 4096: 768 / 571 us, 4000 x 2000 x 2000: 102 / 92 us, 1000 x 2001 x 2001: 44 / 57 us; bf16,
+// 8192 x 4097 x 4096: 689 / 479 us).  Three pieces of fp32 spill there (874 / 1015 us).  Else 128 columns n, and of 384, 256 or 128
+// columns k those that pad K least (K = 270: 384; 131072 rows of fp32, N = 128).
 struct WgPlan { int tk, tn, split; };
 WgPlan wgrad_plan(int64_t M, int N, int K, int dy_dt) {
   auto tiles = [&](int tk, int tn) { return (int64_t)((K + tk - 1) / tk) * ((N + tn - 1) / tn); };
   auto padded = [&](int tk) { return (int64_t)(K + tk - 1) / tk * tk; };
   WgPlan p = {384, 128, 1};
-  if (dy_dt == kBF16 && N % 8 == 0 && tiles(256, 256) >= 64) p = {256, 256, 1};
+  if (tiles(256, 256) >= 64 && (wgrad_direct(N, dy_dt) || (dy_dt != kF32 && M >= 2048))) p = {256, 256, 1};
   else if (padded(256) < padded(384) || padded(128) < padded(384)) p.tk = padded(256) <= padded(128) ? 256 : 128;
   // A stage of 64 rows costs about 2 us where few workgroups run, a split's partial sums N K 8 bytes at 4 TB/s: sqrt of the ratio,
   // as long as the workgroups it makes find a free CU.
@@ -696,6 +703,8 @@ WgPlan wgrad_plan(int64_t M, int N, int K, int dy_dt) {
 
 template <typename T, int P, int ROWS>
 void wgrad(const WgPlan& p, const dim3& grid, const Wg& G, hipStream_t st) {
+  if constexpr (P < 3)
+    if (p.tn == 256) { fp8_wgrad_kernel<T, P, 256, 256, 32, 2, 4, false><<<grid, 512, 0, st>>>(G); return; }
   if (p.tk == 384) fp8_wgrad_kernel<T, P, 384, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
   else if (p.tk == 256) fp8_wgrad_kernel<T, P, 256, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
   else fp8_wgrad_kernel<T, P, 128, 128, ROWS, 4, 2, false><<<grid, 512, 0, st>>>(G);
@@ -811,7 +820,7 @@ int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t
   hipStream_t st = (hipStream_t)stream;
   if (dy_dtype == kF32) wgrad<float, 3, 32>(p, grid, G, st);
   else if (dy_dtype == kF16) wgrad<_Float16, 2, 32>(p, grid, G, st);
-  else if (p.tn == 256) fp8_wgrad_kernel<__bf16, 1, 256, 256, 64, 2, 4, true><<<grid, 512, 0, st>>>(G);
+  else if (p.tn == 256 && wgrad_direct(N, dy_dtype)) fp8_wgrad_kernel<__bf16, 1, 256, 256, 64, 2, 4, true><<<grid, 512, 0, st>>>(G);
   else wgrad<__bf16, 1, 64>(p, grid, G, st);
   HCM_CHECK_LAUNCH();
   if (p.split > 1) return join({G.part, p.split, G.stride, (int64_t)N * K, N, N, nullptr, 0, dw, dw_dtype, db, db_dtype}, st);

@@ -89,6 +89,13 @@ def test_every_tile_and_split(M, N, K):
         _check_step(x, w, None, dy, _run(x, w, None, dy))
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,N,K', [(2100, 2001, 1800), (2049, 2901, 2889)])
+def test_wide_gradient_through_registers(M, N, K, dtype):
+    x, w, b, dy = _inputs(M, N, K, dtype, 8)
+    _check_step(x, w, b, dy, _run(x, w, b, dy))
+
+
 def test_gradient_that_begins_anywhere():
     from hcmoco_amd import hip_ops
     x, w, b, dy = _inputs(300, 96, 200, torch.bfloat16, 6)
