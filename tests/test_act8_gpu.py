@@ -137,3 +137,44 @@ def test_refuses():
         hip_ops.act8_unpack(hip_ops.Act8(p.q[:2], p.scale, p.shape, p.dtype))
     with pytest.raises(ValueError):
         hip_ops.act8_unpack(hip_ops.Act8(p.q, p.scale, (4, 400), p.dtype))
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^32 values: the last rows come out as they do by themselves.  Whole numbers, whose products' sums are
+    exact in any order."""
+    from hcmoco_amd import hip_ops
+    M, C, last = (1 << 20) + 3001, 4096, 300
+    if torch.cuda.mem_get_info()[0] < 110 << 30:
+        pytest.skip('needs 110 GB of device memory')
+    x = torch.randint(-3, 4, (M, C), device=DEV, dtype=torch.bfloat16)
+    tail = x[-last:].clone()
+    packed, small = hip_ops.act8_pack(x), hip_ops.act8_pack(tail)
+    assert torch.equal(packed.q[-last:], small.q) and torch.equal(packed.scale[-last:], small.scale)
+    assert torch.equal(hip_ops.act8_unpack(packed)[-last:], tail)
+    del packed
+
+    w = torch.randint(-2, 3, (C, C), device=DEV, dtype=torch.bfloat16)
+    b = torch.randint(-2, 3, (C,), device=DEV, dtype=torch.bfloat16)
+    dy = torch.zeros_like(x)
+    dy[-last:] = torch.randint(-2, 3, (last, C), device=DEV, dtype=torch.bfloat16)
+
+    def grads(op, *leaves):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        y = op(*leaves)
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy[-leaves[0].shape[0]:]))
+    for act8 in (False, True, None):
+        op = hip_ops.fp8_linear if act8 is None else (lambda *a: hip_ops.layer_norm(*a, act8=act8))
+        p = (w if act8 is None else w[0].contiguous(), b)
+        big, little = grads(op, x, *p), grads(op, tail, *p)
+        for k in (0, 1):
+            assert torch.equal(big[k][-last:], little[k]), (act8, k)
+        for k in (2, 3):
+            if act8 is None:
+                assert torch.equal(big[k], little[k]), k
+            else:       # sums of 300 rows in another order (2^-24 a step), then bf16
+                mag = dy[-last:].double().abs().sum(0) * (1 if k == 3 else 4096 ** 0.5)
+                err = 300 * 2.0 ** -24 * mag + 2.0 ** -8 * little[k].double().abs() * 2
+                assert bool(((big[k].double() - little[k].double()).abs() <= err).all()), (act8, k)
+        del big, little
+    del x, dy, tail
+    torch.cuda.empty_cache()
