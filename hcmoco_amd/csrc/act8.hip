@@ -139,9 +139,10 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const T* __restrict__ w
   }
 }
 
+// rows * kb < 2^30: four threads a block of 128, and a launch has fewer than 2^32
 bool shape_ok(int64_t rows, int cols, int64_t ldq, int64_t lds) {
   const int64_t kb = ((int64_t)cols + 127) / 128;
-  return rows > 0 && cols > 0 && cols <= INT32_MAX - 128 && rows * kb < (1ll << 31) && ldq == ((int64_t)cols + 15) / 16 * 16 && lds == (kb + 3) / 4 * 4;
+  return rows > 0 && cols > 0 && cols <= INT32_MAX - 128 && rows <= INT32_MAX && rows * kb < (1ll << 30) && ldq == ((int64_t)cols + 15) / 16 * 16 && lds == (kb + 3) / 4 * 4;
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

@@ -760,7 +760,7 @@ int hcm_fp8_matmul(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_
   P.split = p.split;
   if (p.split > 1) P.part = (float*)workspace;
   const int64_t tiles = (int64_t)((M + p.tile - 1) / p.tile) * ((N + p.tile - 1) / p.tile);
-  if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
+  if (tiles * (p.tile == 256 ? 512 : 256) >= (1ll << 32)) return (int)hipErrorInvalidValue;       // threads of a launch
   const dim3 grid((uint32_t)tiles, 1, p.split);
   // Four stages keep a long contraction fed where each CU has no more workgroups than fit beside each other with them (one of 128-wide
   // tiles, two of 64: 500 x 4096 x 4096 in bf16 21.8 -> 17.4 us); where it has more, two stages and twice the workgroups at once are
@@ -813,7 +813,7 @@ int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t
   const WgPlan p = wgrad_plan(M, N, K, dy_dtype);
   if (p.split > 1 && (!workspace || workspace_bytes < hcm_fp8_wgrad_workspace_bytes(M, N, K, dy_dtype, dw != nullptr))) return (int)hipErrorInvalidValue;
   const int64_t tiles = (int64_t)((K + p.tk - 1) / p.tk) * ((N + p.tn - 1) / p.tn), steps = (M + kWgRows - 1) / kWgRows;
-  if (tiles >= (1ll << 31)) return (int)hipErrorInvalidValue;
+  if (tiles * 512 >= (1ll << 32)) return (int)hipErrorInvalidValue;       // threads of a launch
   const Wg G = {x,  x_scale, ldx, ldsx, dy, M, N, K, (steps + p.split - 1) / p.split * kWgRows, p.split > 1 ? (float*)workspace : nullptr, wgrad_stride(N, K),
                 dw, db,      dw_dtype, db_dtype};
   const dim3 grid((uint32_t)tiles, 1, p.split);

@@ -443,6 +443,10 @@ int bwd(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t
   return 0;
 }
 
+// what a launch of fewer than 2^32 threads covers: 32 threads a column in norm_reduce_kernel, kLong a row too long for registers
+bool size_ok(int64_t rows, int cols) {
+  return rows > 0 && rows < (1ll << 31) - 8192 && cols > 0 && cols < (1 << 27) && (cols <= kRegCols || rows < (1ll << 32) / kLong);
+}
 bool dt_ok(int d) { return d == kF32 || d == kBF16 || d == kF16; }
 bool pitches_ok(int cols, int64_t ldq, int64_t lds) { return ldq == hcm_act8_pitch(cols) && lds == hcm_act8_scale_pitch(cols); }
 
@@ -452,7 +456,7 @@ extern "C" {
 
 int hcm_layer_norm_forward(const void* x, int dtype, int64_t rows, int cols, int64_t ldx, const void* w, int w_dtype, const void* b, int b_dtype,
                            float eps, void* y, float* mean, float* rstd, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, hcm_stream_t stream) {
-  if (!x || !y || rows <= 0 || rows >= (1ll << 31) - 8192 || cols <= 0 || cols > INT32_MAX - 16384 || ldx < cols || !dt_ok(dtype) || !dt_ok(w_dtype) ||
+  if (!x || !y || !size_ok(rows, cols) || ldx < cols || !dt_ok(dtype) || !dt_ok(w_dtype) ||
       !dt_ok(b_dtype) || (!mean != !rstd) || (!q != !scale) || (q && (!pitches_ok(cols, ldq, lds) || ((uintptr_t)q & 15))))
     return (int)hipErrorInvalidValue;
   const Params P = {w, b, w_dtype, b_dtype};
@@ -471,8 +475,8 @@ size_t hcm_layer_norm_backward_workspace_bytes(int64_t rows, int cols) {
 int hcm_layer_norm_backward(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, const void* dy, int dtype,
                             int64_t rows, int cols, const void* w, int w_dtype, const float* mean, const float* rstd, void* dx, void* dw, void* db,
                             int b_dtype, void* workspace, size_t workspace_bytes, hcm_stream_t stream) {
-  if ((!x == !q) || (!q != !scale) || !dy || !mean || !rstd || !dx || !workspace || rows <= 0 || rows >= (1ll << 31) - 8192 || cols <= 0 ||
-      cols > INT32_MAX - 16384 || (x && ldx < cols) || !dt_ok(dtype) || !dt_ok(w_dtype) || !dt_ok(b_dtype) ||
+  if ((!x == !q) || (!q != !scale) || !dy || !mean || !rstd || !dx || !workspace || !size_ok(rows, cols) ||
+      (x && ldx < cols) || !dt_ok(dtype) || !dt_ok(w_dtype) || !dt_ok(b_dtype) ||
       (q && (!pitches_ok(cols, ldq, lds) || ((uintptr_t)q & 15))) || workspace_bytes < hcm_layer_norm_backward_workspace_bytes(rows, cols))
     return (int)hipErrorInvalidValue;
   const Params P = {w, nullptr, w_dtype, b_dtype};

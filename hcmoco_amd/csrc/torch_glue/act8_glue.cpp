@@ -56,8 +56,8 @@ struct Rows { Tensor t; int64_t rows, ld; int cols; };
 Rows rows_of(const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, name, ": the last axis must have at least one element");
   const int64_t cols = x.size(-1), rows = x.numel() / cols;
-  TORCH_CHECK_VALUE(cols <= INT32_MAX - 16384 && rows * ((cols + 127) / 128) < (1ll << 31) - 8192, name, ": ", rows, " rows of ", cols,
-                    " values are too many (blocks of 128 are numbered in 31 bits)");
+  TORCH_CHECK_VALUE(cols <= INT32_MAX - 16384 && rows < (1ll << 31) - 8192 && rows * ((cols + 127) / 128) < (1ll << 30), name, ": ", rows, " rows of ", cols,
+                    " values are too many (at most 2^30 blocks of 128)");
   if (x.is_contiguous()) return {x, rows, cols, (int)cols};
   if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= cols) return {x, rows, x.stride(0), (int)cols};
   return {x.contiguous(), rows, cols, (int)cols};
@@ -205,6 +205,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   TORCH_CHECK_VALUE(x.dim() > 0, "layer_norm: x needs at least one axis");
   check_vector(w, x, x.size(-1), "layer_norm", "weight");
   check_vector(b, x, x.size(-1), "layer_norm", "bias");
+  TORCH_CHECK_VALUE(x.size(-1) < (1 << 27), "layer_norm: rows of at most 2^27 - 1 values, got ", x.size(-1));
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
   const c10::DeviceGuard guard(x.device());
   if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) return norm_forward(x, w, b, eps, false, false).y;

@@ -90,6 +90,18 @@ def test_products_refuse():
         assert L.hcm_fp8_wgrad(*[a[k] for k in good], Z) != 0, bad
 
 
+def test_sizes_past_a_launch_are_refused():
+    L, bad = _lib.lib(), 1      # hipErrorInvalidValue, not a launch that the runtime turned down
+    assert L.hcm_act8_pack(P, 0, 2 ** 30, 1, 1, P, 16, P, 4, Z) == bad
+    assert L.hcm_act8_unpack(P, 16, P, 4, 2 ** 30, 1, P, 0, Z) == bad
+    for rows, cols in ((1, 2 ** 27), (2 ** 22, 16385)):
+        assert L.hcm_layer_norm_forward(P, 0, rows, cols, cols, Z, 0, Z, 0, 1e-5, P, P, P, Z, 0, Z, 0, Z) == bad
+        n = L.hcm_layer_norm_backward_workspace_bytes(rows, cols)
+        assert L.hcm_layer_norm_backward(P, cols, Z, 0, Z, 0, P, 0, rows, cols, Z, 0, P, P, P, P, P, 0, P, n, Z) == bad
+    M, N, K = 2 ** 31 - 1000, 2 ** 22, 128
+    assert L.hcm_fp8_matmul(P, 128, P, 4, P, 128, P, 4, Z, 0, M, N, K, P, 1, P, 1 << 60, Z) == bad
+
+
 def test_the_format_of_the_reference_matches_torchs_e4m3():
     g = torch.Generator().manual_seed(0)
     x = torch.randn(50, 300, generator=g) * torch.exp(4 * torch.randn(50, 1, generator=g))
