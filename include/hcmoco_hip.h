@@ -766,8 +766,9 @@ int hcm_fp8_wgrad(const uint8_t* x, int64_t ldx, const uint8_t* x_scale, int64_t
                   int K, void* dw, int dw_dtype, void* db, int db_dtype, void* workspace, size_t workspace_bytes, hcm_stream_t stream);
 
 /* Layer norm over the last axis: y [rows, cols] = (x - mean) / sqrt(var + eps) * w + b; sums in fp32.  w, b: NULL = 1, 0.
- * mean, rstd [rows] fp32: NULL when no backward pass follows. cols < 2^27; rows < 2^22 beyond 16384 columns.  q, scale: NULL, or the 8-bit checkpoint of x is written too.
- * Backward takes either x or its checkpoint (the other NULL); dw, db: NULL = not wanted; fixed order, no atomics. */
+ * mean, rstd [rows] fp32: NULL when no backward pass follows.  q, scale: NULL, or the 8-bit checkpoint of x is written too.
+ * Backward takes either x or its checkpoint (the other NULL); dw, db: NULL = not wanted; fixed order, no atomics.
+ * cols < 2^27; rows < 2^22 beyond 16384 columns. */
 int hcm_layer_norm_forward(const void* x, int dtype, int64_t rows, int cols, int64_t ldx, const void* w, int w_dtype, const void* b,
                            int b_dtype, float eps, void* y, float* mean, float* rstd, uint8_t* q, int64_t ldq, uint8_t* scale,
                            int64_t lds, hcm_stream_t stream);
