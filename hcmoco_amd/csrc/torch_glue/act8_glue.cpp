@@ -79,6 +79,19 @@ Tensor workspace(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
 }
 
+// What the backward pass gets back of a tensor it saved.  A saved-tensor hook may return it in another layout, on other memory
+// (save_on_cpu: a contiguous copy of what was a column slice), so nothing but the size is taken from the forward pass, and that is checked.
+Tensor restored(const Tensor& t, at::ScalarType dtype, at::IntArrayRef sizes, const Tensor& dy, const char* name) {
+  TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.scalar_type() == dtype && t.sizes() == sizes && t.device() == dy.device(), name,
+              ": a saved tensor of type ", dtype, " and size ", sizes, " on ", dy.device(), " came back from its hook as something else");
+  return t;
+}
+// the same for a buffer, as it was allocated: contiguous, the 8-bit ones on a 16-byte border
+Tensor restored_buffer(const Tensor& t, at::ScalarType dtype, at::IntArrayRef sizes, const Tensor& dy, const char* name) {
+  const Tensor c = restored(t, dtype, sizes, dy, name).contiguous();
+  return dtype == at::kByte && ((uintptr_t)c.data_ptr() & 15) ? c.clone() : c;
+}
+
 // A backward pass that is itself recorded (create_graph) has no second derivative: asking for one raises.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -154,22 +167,32 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     NormOut o = norm_forward(x, w, b, eps, true, act8);
     const bool nx = x.requires_grad(), nw = w.defined() && w.requires_grad(), nb = b.defined() && b.requires_grad();
     ctx->save_for_backward({o.a, o.scale, o.stats, w});
-    ctx->saved_data["m"] = std::vector<int64_t>{o.r.rows, o.r.cols, o.r.ld, act8, nx, nw, nb, b.defined() ? (int64_t)b.scalar_type() : 0};
+    ctx->saved_data["m"] = std::vector<int64_t>{o.r.rows, o.r.cols, act8, nx, nw, nb, w.defined() ? (int64_t)w.scalar_type() : -1,
+                                                b.defined() ? (int64_t)b.scalar_type() : 0};
     return o.y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &a = saved[0], &scale = saved[1], &stats = saved[2], &w = saved[3];
     const auto m = ctx->saved_data["m"].toIntVector();
-    const int64_t rows = m[0], ld = m[2];
+    const int64_t rows = m[0];
     const int cols = (int)m[1];
-    const bool act8 = m[3], nx = m[4], nw = m[5], nb = m[6];
+    const bool act8 = m[2], nx = m[3], nw = m[4], nb = m[5];
     Tensor dx, dw, db;
     {
       at::AutoGradMode off(false);
       const Tensor dy = grads[0].contiguous();
       const c10::DeviceGuard guard(dy.device());
+      Rows x{};
+      Packed p;
+      if (act8) {
+        p.q = restored_buffer(saved[0], at::kByte, {rows, hcm_act8_pitch(cols)}, dy, "layer_norm");
+        p.scale = restored_buffer(saved[1], at::kByte, {rows, hcm_act8_scale_pitch(cols)}, dy, "layer_norm");
+      } else {
+        x = rows_of(restored(saved[0], dy.scalar_type(), dy.sizes(), dy, "layer_norm"), "layer_norm");
+      }
+      const Tensor stats = restored_buffer(saved[2], at::kFloat, {2, rows}, dy, "layer_norm");
+      const Tensor w = m[6] < 0 ? Tensor() : restored_buffer(saved[3], (at::ScalarType)m[6], {cols}, dy, "layer_norm");
       dx = at::empty_like(dy);
       if (nw) dw = at::empty({cols}, w.options());
       if (nb) db = at::empty({cols}, dy.options().dtype((at::ScalarType)m[7]));
@@ -177,9 +200,9 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         const size_t n = hcm_layer_norm_backward_workspace_bytes(rows, cols);
         const Tensor ws = workspace(n, dy);
         const float* st = stats.data_ptr<float>();
-        check_rc(hcm_layer_norm_backward(act8 ? nullptr : a.data_ptr(), ld, act8 ? bytes(a) : nullptr, act8 ? a.size(1) : 0, bytes(scale),
-                                         act8 ? scale.size(1) : 0, dy.data_ptr(), dt_of(dy, "layer_norm"), rows, cols, ptr(w), dt_of(w, "layer_norm"), st,
-                                         st + rows, dx.data_ptr(), ptr(dw), ptr(db), dt_of(db, "layer_norm"), ptr(ws), n, stream_of(dy)),
+        check_rc(hcm_layer_norm_backward(ptr(x.t), x.ld, bytes(p.q), act8 ? p.q.size(1) : 0, bytes(p.scale), act8 ? p.scale.size(1) : 0, dy.data_ptr(),
+                                         dt_of(dy, "layer_norm"), rows, cols, ptr(w), dt_of(w, "layer_norm"), st, st + rows, dx.data_ptr(), ptr(dw), ptr(db),
+                                         dt_of(db, "layer_norm"), ptr(ws), n, stream_of(dy)),
                  "hcm_layer_norm_backward");
       } else {
         if (nw) dw.zero_();
@@ -284,6 +307,9 @@ struct Weight8 {
   Tensor first, second;              // what the backward pass keeps: the buffer; or qt and scale_t
   const uint8_t *q, *scale, *qt, *scale_t;
 };
+int64_t weight_bytes(int64_t N, int64_t K) {
+  return N * hcm_act8_pitch(K) + K * hcm_act8_pitch(N) + (N + 127) / 128 * hcm_act8_scale_pitch(K) + (K + 127) / 128 * hcm_act8_scale_pitch(N);
+}
 Weight8 weight_in(const Tensor& buffer, int64_t N, int64_t K) {
   Weight8 w;
   w.first = buffer;
@@ -297,8 +323,7 @@ Weight8 lay_out(const Tensor& weight) {
   const Rows r = rows_of(weight, "fp8_linear");
   const int64_t N = r.rows, K = r.cols;
   TORCH_CHECK_VALUE(N > 0 && N <= kMaxSide && K <= kMaxSide, "fp8_linear: expected a weight [N, K] with both in 1..2^22, got ", weight.sizes());
-  const int64_t size = N * hcm_act8_pitch(K) + K * hcm_act8_pitch(N) + (N + 127) / 128 * hcm_act8_scale_pitch(K) + (K + 127) / 128 * hcm_act8_scale_pitch(N);
-  Weight8 w = weight_in(workspace(size, weight), N, K);
+  Weight8 w = weight_in(workspace(weight_bytes(N, K), weight), N, K);
   check_rc(hcm_fp8_weight_pack(r.t.data_ptr(), dt_of(weight, "fp8_linear"), (int)N, (int)K, r.ld, (uint8_t*)w.q, hcm_act8_pitch(K), (uint8_t*)w.scale,
                                hcm_act8_scale_pitch(K), (uint8_t*)w.qt, hcm_act8_pitch(N), (uint8_t*)w.scale_t, hcm_act8_scale_pitch(N), stream_of(weight)),
            "hcm_fp8_weight_pack");
@@ -338,7 +363,8 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     Tensor y = linear_forward(r, W.q, W.scale, N, b, with_last(x.sizes(), N), nw ? &packed : nullptr);
     // x itself is not kept: the 8-bit operand of this product is the checkpoint that the weight's gradient reads
     ctx->save_for_backward({packed, nx ? W.first : Tensor(), nx ? W.second : Tensor()});
-    std::vector<int64_t> m{r.rows, N, r.cols, nx, nw, wants_grad(b), nw ? (int64_t)w.scalar_type() : 0, b.defined() ? (int64_t)b.scalar_type() : 0};
+    std::vector<int64_t> m{r.rows, N, r.cols, nx, nw, wants_grad(b), nw ? (int64_t)w.scalar_type() : 0, b.defined() ? (int64_t)b.scalar_type() : 0,
+                           !W.second.defined()};
     m.insert(m.end(), x.sizes().begin(), x.sizes().end());
     ctx->saved_data["m"] = std::move(m);
     return y;
@@ -347,7 +373,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const auto m = ctx->saved_data["m"].toIntVector();
-    const at::IntArrayRef shape(m.data() + 8, m.size() - 8);
+    const at::IntArrayRef shape(m.data() + 9, m.size() - 9);
     const int64_t M = m[0], N = m[1], K = m[2];
     const bool nx = m[3], nw = m[4], nb = m[5];
     Tensor dx, dw, db;
@@ -358,8 +384,14 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       const c10::DeviceGuard guard(dy.device());
       if (nx) {
         Weight8 W;
-        if (saved[2].defined()) W.qt = bytes(saved[1]), W.scale_t = bytes(saved[2]);
-        else W = weight_in(saved[1], N, K);
+        if (m[8]) {
+          W = weight_in(restored_buffer(saved[1], at::kByte, {weight_bytes(N, K)}, dy, "fp8_linear"), N, K);
+        } else {
+          W.first = restored_buffer(saved[1], at::kByte, {K, hcm_act8_pitch(N)}, dy, "fp8_linear");
+          W.second = restored_buffer(saved[2], at::kByte, {(K + 127) / 128, hcm_act8_scale_pitch(N)}, dy, "fp8_linear");
+          W.qt = bytes(W.first);
+          W.scale_t = bytes(W.second);
+        }
         dx = linear_forward({dy, M, N, (int)N}, W.qt, W.scale_t, K, Tensor(), shape, nullptr);
       }
       if (nw) dw = at::empty({N, K}, dy.options().dtype((at::ScalarType)m[6]));
@@ -368,7 +400,8 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
         const int dt = dt_of(dy, "fp8_linear");
         const size_t n = hcm_fp8_wgrad_workspace_bytes(M, (int)N, (int)K, dt, nw);
         const Tensor work = workspace(n, dy);
-        const uint8_t* q = nw ? bytes(saved[0]) : nullptr;
+        const Tensor packed = nw ? restored_buffer(saved[0], at::kByte, {M * (hcm_act8_pitch(K) + hcm_act8_scale_pitch(K))}, dy, "fp8_linear") : Tensor();
+        const uint8_t* q = bytes(packed);
         check_rc(hcm_fp8_wgrad(q, hcm_act8_pitch(K), nw ? q + M * hcm_act8_pitch(K) : nullptr, hcm_act8_scale_pitch(K), dy.data_ptr(), dt, M, (int)N, (int)K,
                                ptr(dw), dt_of(dw, "fp8_linear"), ptr(db), dt_of(db, "fp8_linear"), ptr(work), n, stream_of(dy)),
                  "hcm_fp8_wgrad");
