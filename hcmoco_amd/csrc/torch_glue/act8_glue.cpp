@@ -4,6 +4,7 @@
 // two directions, more than every kernel of a small batch.  hip_ops.layer_norm / act8_pack / act8_unpack / fp8_* document the
 // operators; the errors raised here are the ones they document (TypeError, ValueError, RuntimeError).
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -222,6 +223,14 @@ void check_vector(const Tensor& p, const Tensor& x, int64_t n, const char* name,
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// Forward-mode differentiation: these operators have no rule for it, and a dual tensor that no backward graph records would lose its
+// tangent without a word (a missing tangent reads as zero).
+void check_no_tangent(std::initializer_list<const Tensor*> inputs, const char* name) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
+
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, bool act8) {
   const Tensor w = value(weight), b = value(bias);
   check_float(x, x, "layer_norm");
@@ -230,6 +239,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   check_vector(b, x, x.size(-1), "layer_norm", "bias");
   TORCH_CHECK_VALUE(x.size(-1) < (1 << 27), "layer_norm: rows of at most 2^27 - 1 values, got ", x.size(-1));
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
+  check_no_tangent({&x, &w, &b}, "layer_norm");
   const c10::DeviceGuard guard(x.device());
   if (!at::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(w) || wants_grad(b))) return norm_forward(x, w, b, eps, false, false).y;
   return LayerNorm::apply(x, weight, bias, eps, act8);
@@ -430,6 +440,7 @@ Tensor fp8_linear(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   const int64_t N = w_shape[0];
   check_vector(b, x, N, "fp8_linear", "bias");
   TORCH_CHECK_VALUE(x.numel() / K <= INT32_MAX - 512, "fp8_linear: too many rows");
+  check_no_tangent({&x, &w, &b}, "fp8_linear");
   const c10::DeviceGuard guard(x.device());
   Weight8 W;
   if (w.defined()) {

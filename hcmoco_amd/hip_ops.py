@@ -743,7 +743,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
     as an 8-bit checkpoint (``act8_pack``'s format, written by the same kernel) instead of x itself, and computes its gradients
     from the checkpoint's values with the exact mean and variance: a quarter of the memory for float32, at an error of up to
     2^-4 of |x| in the normalised values that the gradients of weight and x are formed with.  Deterministic; no second
-    derivative."""
+    and no forward-mode derivative (both raise)."""
     return _lib.torch_glue().layer_norm(x, weight, bias, float(eps), bool(act8))
 
 
@@ -785,7 +785,7 @@ def fp8_linear(x, weight, bias=None):
     dx = Q(dy) Q(weight), dweight = dy^T Q(x), dbias = sum of dy.  The backward pass keeps Q(x), a byte a value, and not x; dy enters
     the weight's gradient unrounded.  Q is the format of :func:`act8_pack`: rows of x and dy in blocks of 128, the weight in blocks
     of 128 x 128.  Sums are fp32; for a 16-bit x, y and dx come from the 8-bit matrix instructions, which drop what lies 2^-13 below
-    the largest of eight neighbouring products (2e-5 .. 7e-5 of the result's norm).  Deterministic; no second derivative."""
+    the largest of eight neighbouring products (2e-5 .. 7e-5 of the result's norm).  Deterministic; no second and no forward-mode derivative (both raise)."""
     if isinstance(weight, Fp8Weight):
         return _lib.torch_glue().fp8_linear(x, None, bias, weight.q, weight.scale, weight.qt, weight.scale_t, weight.shape)
     return _lib.torch_glue().fp8_linear(x, weight, bias, None, None, None, None, ())
