@@ -10,6 +10,7 @@
 // twice up to 16384 columns; longer rows walk memory (norm_long_*).  Workgroups stay and take row after row: the parameters are read once,
 // and the column sums of dw and db grow in registers.  They leave as one partial row per workgroup, summed by norm_reduce_kernel in
 // a fixed order (no atomics: the same bits on every run).
+#include <algorithm>
 #include "act8.h"
 #include "../../include/hcmoco_hip.h"
 
@@ -261,6 +262,10 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ x, i
   }
 }
 
+// No fp32 sum here is a chain of more than 2 kChain additions, whatever the size (each can lose half a unit of a sum that has grown that
+// long): what is longer is added up in runs of kChain, and a batch of many rows gets more workgroups or slices, each of at most kChain trips.
+constexpr int kChain = 256;
+
 // out[c] = sum over `parts` rows of part[][c], c < 2 cols: 64 columns a workgroup, 16 slices of the rows, every load of a slice in flight
 constexpr int kRedSlices = 16;
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restrict__ part, int parts, int cols, void* __restrict__ dw, int wdt,
@@ -271,9 +276,14 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
   float a[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < n) {
     int p = slice;
-    for (; p + 3 * kRedSlices < parts; p += 4 * kRedSlices)
+    while (p + 3 * kRedSlices < parts) {
+      float run[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < kChain && p + 3 * kRedSlices < parts; ++k, p += 4 * kRedSlices)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) a[u] += part[(int64_t)(p + u * kRedSlices) * n + c];
+        for (int u = 0; u < 4; ++u) run[u] += part[(int64_t)(p + u * kRedSlices) * n + c];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a[u] += run[u];
+    }
     for (; p < parts; p += kRedSlices) a[0] += part[(int64_t)p * n + c];
   }
   s[slice][lane] = (a[0] + a[1]) + (a[2] + a[3]);
@@ -300,6 +310,20 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return s;
 }
 
+// sum of term(c) over this thread's columns, in runs (term adds to what it is given)
+template <int N, typename Term>
+__device__ __forceinline__ void lane_sums(int cols, float (&s)[N], Term term) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) s[n] = 0.f;
+  for (int64_t c0 = threadIdx.x; c0 < cols; c0 += (int64_t)kChain * kLong) {
+    const int64_t end = min((int64_t)cols, c0 + (int64_t)kChain * kLong);
+    float run[N] = {};
+    for (int64_t c = c0; c < end; c += kLong) term(c, run);
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] += run[n];
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kLong) void norm_long_fwd_kernel(const T* __restrict__ x, int64_t ldx, int cols, Params P, float eps, T* __restrict__ y,
                                                               float* __restrict__ mean_out, float* __restrict__ rstd_out, uint8_t* __restrict__ q,
@@ -307,15 +331,14 @@ __global__ __launch_bounds__(kLong) void norm_long_fwd_kernel(const T* __restric
   __shared__ float red[kLong / 64];
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
-  float s = 0.f;
-  for (int64_t c = threadIdx.x; c < cols; c += kLong) s += (float)xr[c];
-  const float mean = block_sum(s, red) / (float)cols;
-  s = 0.f;
-  for (int64_t c = threadIdx.x; c < cols; c += kLong) {
+  float s[1];
+  lane_sums(cols, s, [&](int64_t c, float (&run)[1]) { run[0] += (float)xr[c]; });
+  const float mean = block_sum(s[0], red) / (float)cols;
+  lane_sums(cols, s, [&](int64_t c, float (&run)[1]) {
     const float d = (float)xr[c] - mean;
-    s = fmaf(d, d, s);
-  }
-  const float rstd = 1.f / sqrtf(block_sum(s, red) / (float)cols + eps);
+    run[0] = fmaf(d, d, run[0]);
+  });
+  const float rstd = 1.f / sqrtf(block_sum(s[0], red) / (float)cols + eps);
   for (int64_t c = threadIdx.x; c < cols; c += kLong) {
     const float w = P.w ? load_dt(P.w, P.wdt, c) : 1.f, b = P.b ? load_dt(P.b, P.bdt, c) : 0.f;
     y[row * cols + c] = (T)fmaf(((float)xr[c] - mean) * rstd, w, b);
@@ -353,13 +376,13 @@ __global__ __launch_bounds__(kLong) void norm_long_bwd_kernel(const T* __restric
   const T *xr = ACT8 ? nullptr : x + row * ldx, *dr = dy + row * cols;
   const uint8_t *qr = ACT8 ? q + row * ldq : nullptr, *sr = ACT8 ? scale + row * lds : nullptr;
   const float mean = mean_in[row], rstd = rstd_in[row];
-  float s0 = 0.f, s1 = 0.f;
-  for (int64_t c = threadIdx.x; c < cols; c += kLong) {
+  float s[2];
+  lane_sums(cols, s, [&](int64_t c, float (&run)[2]) {
     const float g = (float)dr[c] * (P.w ? load_dt(P.w, P.wdt, c) : 1.f);
-    s0 += g;
-    s1 = fmaf(g, (long_x<T, ACT8>(xr, qr, sr, c) - mean) * rstd, s1);
-  }
-  const float mg = block_sum(s0, red) / (float)cols, mgh = block_sum(s1, red) / (float)cols;
+    run[0] += g;
+    run[1] = fmaf(g, (long_x<T, ACT8>(xr, qr, sr, c) - mean) * rstd, run[1]);
+  });
+  const float mg = block_sum(s[0], red) / (float)cols, mgh = block_sum(s[1], red) / (float)cols;
   for (int64_t c = threadIdx.x; c < cols; c += kLong) {
     const float g = (float)dr[c] * (P.w ? load_dt(P.w, P.wdt, c) : 1.f);
     dx[row * cols + c] = (T)(rstd * (g - mg - (long_x<T, ACT8>(xr, qr, sr, c) - mean) * rstd * mgh));
@@ -389,10 +412,12 @@ __global__ __launch_bounds__(256) void norm_long_cols_kernel(const T* __restrict
   X(16, 1, 256) X(16, 3, 256) X(64, 1, 256) X(64, 2, 256) X(64, 4, 256) X(256, 2, 256) X(256, 4, 256) X(512, 4, 512)
 
 constexpr int kRegCols = 16384;
-constexpr int kLongSlices = 32;
+
+// slices of the rows in norm_long_cols_kernel
+int long_slices(int64_t rows) { return (int)std::max(std::min(rows, (int64_t)32), (rows + kChain - 1) / kChain); }
 
 // Workgroups of the backward pass: as many as run at once; each costs a partial row of 2 * cols floats, so wide rows get fewer (8192 x 8000 in
-// fp32: 116 us with 256, 126 with 512).
+// fp32: 116 us with 256, 126 with 512).  More only where one would make over kChain trips.
 int bwd_groups(int64_t rows, int cols) {
   int64_t per = 1;
   const int cap = cols <= 384 ? 1024 : cols <= 4096 ? 512 : 256;
@@ -400,7 +425,7 @@ int bwd_groups(int64_t rows, int cols) {
   HCM_NORM_SHAPES(X)
 #undef X
   const int64_t need = (rows + per - 1) / per;
-  return (int)(need < cap ? need : cap);
+  return (int)std::max(std::min(need, (int64_t)cap), (need + kChain - 1) / kChain);
 }
 
 template <typename T>
@@ -436,7 +461,7 @@ int bwd(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t
 #undef X
   norm_long_bwd_kernel<T, ACT8><<<(uint32_t)rows, kLong, 0, st>>>((const T*)x, ldx, q, ldq, scale, lds, (const T*)dy, cols, P, mean, rstd, (T*)dx);
   HCM_CHECK_LAUNCH();
-  parts = (int)(rows < kLongSlices ? rows : kLongSlices);
+  parts = long_slices(rows);
   norm_long_cols_kernel<T, ACT8><<<dim3((cols + 255) / 256, parts), 256, 0, st>>>((const T*)x, ldx, q, ldq, scale, lds, (const T*)dy, rows, cols, mean, rstd,
                                                                                   part);
   HCM_CHECK_LAUNCH();
@@ -468,7 +493,7 @@ int hcm_layer_norm_forward(const void* x, int dtype, int64_t rows, int cols, int
 
 size_t hcm_layer_norm_backward_workspace_bytes(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int64_t parts = cols > kRegCols ? (rows < kLongSlices ? rows : kLongSlices) : bwd_groups(rows, cols);
+  const int64_t parts = cols > kRegCols ? long_slices(rows) : bwd_groups(rows, cols);
   return (size_t)parts * 2 * cols * sizeof(float);
 }
 

@@ -1,0 +1,53 @@
+"""hip_ops.layer_norm at the sizes where its sums get long: very long rows, and more rows than its workgroups hold at once.
+
+Tolerances: u = 2^-24.  No sum in the kernels is a chain of more than 256 additions of terms, and what those make is added up again
+(at most 64 of them here, then 22 more in a tree of lanes, waves and slices): a sum is off by at most 350 u sum|terms|."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda:0'
+U = 2.0 ** -24
+SUM = 350 * U
+
+
+def _needs(gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes << 30:
+        pytest.skip('needs %d GB of device memory' % gigabytes)
+
+
+def test_sums_along_a_very_long_row():
+    """Equal values, just above a power of two: a running sum of 16384 of them (2^24 columns on 1024 lanes) would round each one down and
+    lose 2e-4 of itself.  With eps = 1: y = x - mean = 0 up to the mean's error, and dx = dy - mean(dy) = 0 likewise."""
+    from hcmoco_amd import hip_ops
+    C = 1 << 24
+    x = torch.full((1, C), 1 + 0.9 * 2.0 ** -11, device=DEV, requires_grad=True)
+    y = hip_ops.layer_norm(x, eps=1.0)
+    assert float(y.detach().abs().max()) <= 2 * SUM
+    dx, = torch.autograd.grad(y, x, torch.full_like(y, 1 + 0.9 * 2.0 ** -11))
+    assert float(dx.abs().max()) <= 2 * SUM
+    # and the variance: (x - mean)^2 = (1 + 0.9 * 2^-11)^2 in every column
+    s = (1 + 0.9 * 2.0 ** -11) * (1 - 2 * (torch.arange(C, device=DEV) & 1).float())
+    y = hip_ops.layer_norm(s[None], eps=0.0)
+    assert float((y.abs() - 1).abs().max()) <= 2 * SUM
+
+
+@pytest.mark.parametrize('rows,cols,memory', [(200000, 16385, 100), (1000000, 4100, 110), (3000000, 400, 40)])
+def test_sums_over_very_many_rows(rows, cols, memory):
+    """dy of one value whose running sum, over 2048 long, would round each addition down (7e-5 of the sum at 200000 rows).  x is +1 and
+    -1 in turn along every row, so that h is +-1/2 and dw sums equal terms too."""
+    from hcmoco_amd import hip_ops
+    _needs(memory)
+    eps = 3.0                                               # sqrt(1 + 3) = 2: h is exactly +-1/2
+    cols += cols & 1
+    v = 1 + 0.9 * 2.0 ** -13
+    x = torch.ones(rows, cols, device=DEV)
+    x[:, 1::2] = -1
+    w, b = torch.ones(cols, device=DEV, requires_grad=True), torch.zeros(cols, device=DEV, requires_grad=True)
+    y = hip_ops.layer_norm(x, w, b, eps=eps)
+    assert torch.equal(y[-1], 0.5 * x[-1]) and torch.equal(y[rows // 2], 0.5 * x[0])
+    dw, db = torch.autograd.grad(y, (w, b), torch.full((1, 1), v, device=DEV).expand(rows, cols))
+    vf = float(torch.tensor(v))
+    assert float((db.double() - rows * vf).abs().max()) <= (SUM + U) * rows * vf
+    assert float((dw.double() - 0.5 * rows * vf * x[0].double()).abs().max()) <= (SUM + 4 * U) * 0.5 * rows * vf
