@@ -272,7 +272,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* __restri
                                                            void* __restrict__ db, int bdt) {
   __shared__ float s[kRedSlices][64];
   const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane, n = 2ll * cols;
+  const int64_t c = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 64 + lane, n = 2ll * cols;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < n) {
     int p = slice;
@@ -468,7 +468,7 @@ int bwd(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t
   return 0;
 }
 
-// what a launch of fewer than 2^32 threads covers: 32 threads a column in norm_reduce_kernel, kLong a row too long for registers
+// what launches of fewer than 2^32 threads an axis cover: kLong threads a row that is too long for registers
 bool size_ok(int64_t rows, int cols) {
   return rows > 0 && rows < (1ll << 31) - 8192 && cols > 0 && cols < (1 << 27) && (cols <= kRegCols || rows < (1ll << 32) / kLong);
 }
@@ -518,7 +518,10 @@ int hcm_layer_norm_backward(const void* x, int64_t ldx, const uint8_t* q, int64_
     rc = q ? bwd<_Float16, true>(x, ldx, q, ldq, scale, lds, dy, rows, cols, P, mean, rstd, dx, part, parts, st)
            : bwd<_Float16, false>(x, ldx, q, ldq, scale, lds, dy, rows, cols, P, mean, rstd, dx, part, parts, st);
   if (rc || (!dw && !db)) return rc;
-  norm_reduce_kernel<<<(uint32_t)((2ll * cols + 63) / 64), 64 * kRedSlices, 0, st>>>(part, parts, cols, dw, w_dtype, db, b_dtype);
+  // in two axes: the 32 threads a column would be 2^32 in one for the longest rows
+  const int64_t groups = (2ll * cols + 63) / 64;
+  norm_reduce_kernel<<<dim3((uint32_t)std::min(groups, (int64_t)1 << 16), (uint32_t)((groups + 65535) >> 16)), 64 * kRedSlices, 0, st>>>(part, parts, cols, dw,
+                                                                                                                                     w_dtype, db, b_dtype);
   HCM_CHECK_LAUNCH();
   return 0;
 }

@@ -238,6 +238,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
   check_vector(w, x, x.size(-1), "layer_norm", "weight");
   check_vector(b, x, x.size(-1), "layer_norm", "bias");
   TORCH_CHECK_VALUE(x.size(-1) < (1 << 27), "layer_norm: rows of at most 2^27 - 1 values, got ", x.size(-1));
+  TORCH_CHECK_VALUE(x.size(-1) <= 16384 || x.numel() / x.size(-1) < (1 << 22), "layer_norm: fewer than 2^22 rows of over 16384 values, got ",
+                    x.numel() / x.size(-1));
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
   check_no_tangent({&x, &w, &b}, "layer_norm");
   const c10::DeviceGuard guard(x.device());

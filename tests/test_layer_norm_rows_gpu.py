@@ -12,6 +12,12 @@ U = 2.0 ** -24
 SUM = 350 * U
 
 
+@pytest.fixture(autouse=True)
+def _memory_goes_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 def _needs(gigabytes):
     if torch.cuda.mem_get_info()[0] < gigabytes << 30:
         pytest.skip('needs %d GB of device memory' % gigabytes)
@@ -51,3 +57,41 @@ def test_sums_over_very_many_rows(rows, cols, memory):
     vf = float(torch.tensor(v))
     assert float((db.double() - rows * vf).abs().max()) <= (SUM + U) * rows * vf
     assert float((dw.double() - 0.5 * rows * vf * x[0].double()).abs().max()) <= (SUM + 4 * U) * 0.5 * rows * vf
+
+
+@pytest.mark.parametrize('act8', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_the_longest_row(dtype, act8):
+    """2^27 - 1 columns, both directions, at the values of a sample of columns; the sums of all in float64."""
+    from hcmoco_amd import hip_ops
+    _needs(30)
+    C = (1 << 27) - 1
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x, dy = (torch.randint(-4, 5, (1, C), generator=g, device=DEV, dtype=torch.int8).to(dtype) for _ in range(2))     # 8-bit values: act8 keeps them
+    w, b = (torch.randint(-4, 5, (C,), generator=g, device=DEV, dtype=torch.int8).float() for _ in range(2))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = hip_ops.layer_norm(*leaves, act8=act8)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    x, dy, w, b = (t.detach().double().view(-1) for t in (x, dy, w, b))
+    mean = x.mean()
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean() + 1e-5)
+    gr = dy * w
+    mg, mgh = gr.mean(), (gr * (x - mean)).mean() * rstd
+    # |h|, |g|, |y| <= 2, 16, 12 and a sum's error of 2 * 256 + 22 additions on mean, variance and both means of the gradient
+    err = 600 * U
+    half = torch.finfo(dtype).eps / 2
+    for at in (slice(0, 5000), slice(C // 2, C // 2 + 5000), slice(C - 5000, C)):
+        h = (x[at] - mean) * rstd
+        want = h * w[at] + b[at]
+        assert float(((y.detach().view(-1)[at].double() - want).abs() - 12 * err - half * want.abs()).max()) <= 0
+        want = rstd * (gr[at] - mg - h * mgh)
+        assert float(((dx.view(-1)[at].double() - want).abs() - 100 * err - half * want.abs()).max()) <= 0
+        assert float((dw[at].double() - dy[at] * h).abs().max()) <= 8 * err
+    assert torch.equal(db.double(), dy)
+
+
+def test_too_many_long_rows_are_refused():
+    from hcmoco_amd import hip_ops
+    for train in (False, True):
+        with pytest.raises(ValueError):
+            hip_ops.layer_norm(torch.zeros(1, 1, device=DEV, dtype=torch.bfloat16, requires_grad=train).expand(1 << 22, 16385))
