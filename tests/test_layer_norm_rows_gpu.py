@@ -95,3 +95,41 @@ def test_too_many_long_rows_are_refused():
     for train in (False, True):
         with pytest.raises(ValueError):
             hip_ops.layer_norm(torch.zeros(1, 1, device=DEV, dtype=torch.bfloat16, requires_grad=train).expand(1 << 22, 16385))
+
+
+# (rows, cols): each of the kernels' widths, with three trips of the forward pass's workgroups and five to nine of the backward pass's, the last
+# one not full.  One trip is 32768 and 16384 rows up to 384 columns, 4096 and 2048 up to 2048, 1024 and 512 up to 4096, 1024 and 256 up to
+# 8192, 512 and 256 up to 16384.
+TRIPS = [(65543, 100), (65601, 270), (81001, 384), (8195, 500), (12200, 1000), (8501, 2000), (2051, 4096), (2900, 3001), (2051, 8000), (1031, 16384)]
+
+
+@pytest.mark.parametrize('act8', [False, True])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('rows,cols', TRIPS)
+def test_workgroups_that_take_many_rows(rows, cols, dtype, act8):
+    """Every row's y and dx and both column sums against float64 (tests/test_layer_norm_gpu.py derives the tolerances: its sums of at
+    most 64 additions hold here too, 9 trips + 16 rows side by side + 1024 partial rows by 64 + 20)."""
+    from act8_ref import held8
+    from test_layer_norm_gpu import _check, _inputs, _run, _truth
+    x, w, b, dy = _inputs(rows, cols, dtype, rows)
+    x8 = held8(x)[0].to(DEV) if act8 else None
+    got = _run(x, w, b, dy, 1e-5, act8)
+    want, err = _truth(*(t.to(DEV) for t in (x, w, b, dy)), 1e-5, x8)
+    for g, t, e, n, d in zip(got, want, err, ('y', 'dx', 'dw', 'db'), (dtype, dtype, torch.float32, torch.float32)):
+        _check(g, t.cpu(), e.cpu(), (n, d))
+
+
+@pytest.mark.parametrize('rows,cols', [(65543, 100), (8195, 500), (2051, 4096)])
+def test_many_rows_of_a_column_slice(rows, cols):
+    """The rows that are loaded ahead lie a pitch apart, and what lies between them is NaN."""
+    from test_layer_norm_gpu import _check, _inputs, _truth
+    from hcmoco_amd import hip_ops
+    x, w, b, dy = (t.to(DEV) for t in _inputs(rows, cols, torch.bfloat16, cols))
+    wide = torch.full((rows, cols + 13), float('nan'), dtype=torch.bfloat16, device=DEV)
+    wide[:, 5:5 + cols] = x
+    leaves = [t.requires_grad_() for t in (wide[:, 5:5 + cols].detach(), w, b)]
+    y = hip_ops.layer_norm(*leaves)
+    got = [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    want, err = _truth(x, w.detach(), b.detach(), dy, 1e-5)
+    for g, t, e, n, d in zip(got, want, err, ('y', 'dx', 'dw', 'db'), (torch.bfloat16, torch.bfloat16, torch.float32, torch.float32)):
+        _check(g, t.cpu(), e.cpu(), (n, d))
