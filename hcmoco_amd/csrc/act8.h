@@ -5,9 +5,10 @@
 //     E = the smallest exponent with max|x| <= 448 * 2^E,  at least -126;  0 for a block without a nonzero value
 //     q = e4m3(x * 2^-E), to nearest, ties to even; a value that is not finite becomes NaN and does not count in the maximum
 // Why a power of two and not max|x| / 448: x * 2^-E and q * 2^E are exact, so the stored value does not depend on the order or
-// the rounding of whatever computes it; q * 2^E is exact in bf16 (3 fraction bits), so a checkpoint enters a bf16 matrix
-// instruction without a second rounding; and the scaled matrix instructions of this chip take exactly this byte.  Cost: up to
-// one binade of e4m3's range of eighteen, none of its precision.
+// the rounding of whatever computes it; q * 2^E is exact in bf16 (3 fraction bits) for -124 <= E <= 119, that is, for blocks whose largest
+// magnitude is in 2^-116 .. 2^127, so that a checkpoint enters a bf16 matrix instruction without a second rounding; and the scaled matrix
+// instructions of this chip take exactly this byte.  (Below: bf16's steps are 2^-133.  Above, E = 120: what rounds up to 256, from 248 * 2^120
+// = 3.3e38 on, is 2^128, infinite in bf16 as in fp32.)  Cost: up to one binade of e4m3's range of eighteen, none of its precision.
 #pragma once
 #include "hcm_common.h"
 

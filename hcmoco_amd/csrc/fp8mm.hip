@@ -11,8 +11,8 @@
 // group's largest product, and drops what lies below 2^-13 of it (measured on single products, the same for the scaled form and for
 // 16x16x32; the sums of groups are full fp32): 2e-5 .. 7e-5 of the result's norm on random data.  That is under the rounding of
 // a 16-bit y (2^-9, 2^-12), and it is over that of an fp32 one, so y in fp32 takes the WIDE form: the 8-bit values are widened to bf16
-// on their way from LDS -- exact, the scales included, by v_cvt_scalef32_pk_bf16_fp8 -- and multiplied by v_mfma_f32_16x16x32_bf16,
-// whose sums are fp32 (1e-8 .. 3e-7 on the same data), at half the rate (8192 x 4096 x 4096: 1.33 PFLOP/s; 2.4 in 8 bits).
+// on their way from LDS -- exact in the range of scales that act8.h states, the scales included, by v_cvt_scalef32_pk_bf16_fp8 -- and multiplied
+// by v_mfma_f32_16x16x32_bf16, whose sums are fp32 (1e-8 .. 3e-7 on the same data), at half the rate (8192 x 4096 x 4096: 1.33 PFLOP/s; 2.4 in 8 bits).
 #include <cmath>
 #include "act8.h"
 #include "../../include/hcmoco_hip.h"
@@ -438,7 +438,7 @@ int join(const Join& J, hipStream_t st) {
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Weight gradient from the 8-bit checkpoint:  dW[n][k] = sum_m dy[m][n] X[m][k],  db[n] = sum_m dy[m][n].
 //
-// q * 2^E is exact in bf16, so X enters v_mfma_f32_16x16x32_bf16 without a rounding; dy enters as the bf16 pieces that hold its type
+// q * 2^E is exact in bf16 (act8.h: over nearly all of the range), so X enters v_mfma_f32_16x16x32_bf16 without a rounding; dy enters as the bf16 pieces that hold its type
 // exactly (bf16: 1, fp16: 2, fp32: 3), one instruction a piece: only the fp32 sums round.  Both operands lie row by row (m),
 // and the instruction wants eight m of one column in a lane: the LDS transpose read (lane p of sixteen points at row p / 4, columns
 // 4 (p % 4) .. + 3, and receives column p of the four rows).  128 columns k (one scale a row) x 128 columns n a workgroup.

@@ -722,10 +722,12 @@ class Act8:
 
 
 def act8_pack(x):
-    """``x`` [..., C] (float32 / bfloat16 / float16) -> :class:`Act8`: a byte a value and a byte for 128 of them.  The largest
-    relative error of a value within 2^14 of its block's largest is 2^-4 (half an e4m3 step); what lies further below is held to
-    2^-10 times the block's scale.  Values that are not finite read back as NaN, their neighbours are not disturbed.  Rows may
-    be a column slice of a wider matrix; any other view is copied first."""
+    """``x`` [..., C] (float32 / bfloat16 / float16) -> :class:`Act8`: a byte a value and a byte for 128 of them.  A row takes C
+    bytes rounded up to 16 and 4 more for every 512 values begun, so this is for rows that are long: 1.01 bytes a value at C = 4096, 1.25 at
+    16, 2.5 at 8 (more than bfloat16).  A value is held to max(2^-4 of itself, 2^-10 * 2^E of its block): half an e4m3 step within 2^13
+    of the block's largest value (where that is above 2^-118), and down to nothing far below it.  Values that are not finite read back as NaN, their neighbours are
+    not disturbed.  Rows may be a column slice of a wider matrix; any other view is copied first.  Not differentiable, and neither is
+    :func:`act8_unpack`."""
     q, scale = _lib.torch_glue().act8_pack(x)
     return Act8(q, scale, x.shape, x.dtype)
 
@@ -741,8 +743,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, act8=False):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis, statistics in fp32, differentiable in x, weight and bias
     (any may be float32 / bfloat16 / float16; a gradient has the type of what it belongs to).  ``act8``: the backward pass keeps x
     as an 8-bit checkpoint (``act8_pack``'s format, written by the same kernel) instead of x itself, and computes its gradients
-    from the checkpoint's values with the exact mean and variance: a quarter of the memory for float32, at an error of up to
-    2^-4 of |x| in the normalised values that the gradients of weight and x are formed with.  Deterministic; no second
+    from the checkpoint's values with the exact mean and variance: a quarter of the memory for float32 (``act8_pack`` states the bytes
+    of a short row), at an error of up to max(2^-4 |x|, 2^-10 * 2^E of x's block) / sqrt(var + eps) in the normalised values that
+    the gradients of weight and x are formed with.  Deterministic; no second
     and no forward-mode derivative (both raise)."""
     return _lib.torch_glue().layer_norm(x, weight, bias, float(eps), bool(act8))
 
@@ -764,7 +767,7 @@ class Fp8Weight:
 
 
 def fp8_weight(weight):
-    """``weight`` [N, K] (float32 / bfloat16 / float16) -> :class:`Fp8Weight`, laid out once for any number of products."""
+    """``weight`` [N, K] (float32 / bfloat16 / float16) -> :class:`Fp8Weight`, laid out once for any number of products.  Not differentiable."""
     return Fp8Weight(*_lib.torch_glue().fp8_weight(weight), weight.shape, weight.dtype)
 
 
@@ -783,7 +786,7 @@ def fp8_linear(x, weight, bias=None):
     ``weight``: a tensor, which is laid out anew on every call (training), or an :class:`Fp8Weight` that the caller keeps
     (inference, or a frozen layer).  Differentiable in x, bias and a weight tensor; Q counts as the identity there:
     dx = Q(dy) Q(weight), dweight = dy^T Q(x), dbias = sum of dy.  The backward pass keeps Q(x), a byte a value, and not x; dy enters
-    the weight's gradient unrounded.  Q is the format of :func:`act8_pack`: rows of x and dy in blocks of 128, the weight in blocks
+    the weight's gradient unrounded (what is under 2^-110 to 2^-134).  Q is the format of :func:`act8_pack`: rows of x and dy in blocks of 128, the weight in blocks
     of 128 x 128.  Sums are fp32; for a 16-bit x, y and dx come from the 8-bit matrix instructions, which drop what lies 2^-13 below
     the largest of eight neighbouring products (2e-5 .. 7e-5 of the result's norm).  Deterministic; no second and no forward-mode derivative (both raise)."""
     if isinstance(weight, Fp8Weight):

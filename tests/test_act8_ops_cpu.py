@@ -111,3 +111,18 @@ def test_the_format_of_the_reference_matches_torchs_e4m3():
     assert (x.double() / s).abs().max() <= 448
     blocks = torch.nn.functional.pad((x.double() / s).abs(), (0, 84)).view(50, 3, 128).amax(2)
     assert (blocks > 224).all()                            # a smaller power of two would not have held the block
+
+
+def test_the_bounds_that_act8_pack_states():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(400, 256, generator=g) * torch.exp(4 * torch.randn(400, 256, generator=g))
+    x[0, :2] = torch.tensor([225., 7.5 * 2.0 ** -9])          # within 2^14 of the largest, and off by more than 2^-4 of itself
+    val, e = held8(x)
+    scale = torch.repeat_interleave(torch.exp2(e.double()), 128, 1)
+    off, mag = (val - x.double()).abs(), x.double().abs()
+    assert (off <= torch.maximum(mag / 16, scale / 1024)).all()
+    top = torch.repeat_interleave(mag.view(400, 2, 128).amax(2), 128, 1)
+    assert (off <= mag / 16)[mag * 8192 >= top].all() and off[0, 1] > mag[0, 1] / 16
+    L = _lib.lib()
+    per = lambda c: (L.hcm_act8_pitch(c) + L.hcm_act8_scale_pitch(c)) / c
+    assert (per(8), per(16)) == (2.5, 1.25) and per(4096) < 1.01
