@@ -3,11 +3,7 @@
 # usage (GPU box): strip_timing.sh
 R=${GRAFT_REPO_ROOT:-/root/repo}
 D=/tmp/stripdiag
-rm -rf $D && mkdir -p $D/hcmoco_amd/csrc $D/include && cp $R/include/*.h $D/include/ && cp $R/hcmoco_amd/csrc/*.hip $R/hcmoco_amd/csrc/*.h $D/hcmoco_amd/csrc/ && cd $D/hcmoco_amd/csrc
-for f in *.hip; do
-  extra=""; [ $f = pointnet2.hip ] && extra="-ffp-contract=off -mllvm -amdgpu-atomic-optimizer-strategy=None"; [ $f = scatter.hip ] && extra="-fno-slp-vectorize"; [ $f = bank_lean.hip ] && extra="-fno-slp-vectorize"
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-value -I$R/include -DHCM_STRIP_TIMING $extra -c $f -o ${f%.hip}.o &
-done
-wait
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC *.o -o $D/libhcmoco_hip.so
-HCM_LIB=$D/libhcmoco_hip.so python $R/tools/probes/strip_timing.py
+rm -rf $D && mkdir -p $D/hcmoco_amd/csrc $D/include && cp $R/include/*.h $D/include/ && cp $R/hcmoco_amd/csrc/*.hip $R/hcmoco_amd/csrc/*.h $R/hcmoco_amd/csrc/Makefile $D/hcmoco_amd/csrc/ && cd $D/hcmoco_amd/csrc
+# the product's own rules and flags, with one macro more
+make -s -j16 libhcmoco_hip.so HIPCC="/opt/rocm/bin/hipcc -DHCM_STRIP_TIMING" || exit 1
+HCM_LIB=$D/hcmoco_amd/csrc/libhcmoco_hip.so python $R/tools/probes/strip_timing.py
