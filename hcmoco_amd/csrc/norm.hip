@@ -263,7 +263,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ x, i
 }
 
 // No fp32 sum here is a chain of more than 2 kChain additions, whatever the size (each can lose half a unit of a sum that has grown that
-// long): what is longer is added up in runs of kChain, and a batch of many rows gets more workgroups or slices, each of at most kChain trips.
+// long): what is longer is added up in runs of kChain, and a batch of many rows gets more launches or slices, each of at most kChain trips.
 constexpr int kChain = 256;
 
 // out[c] = sum over `parts` rows of part[][c], c < 2 cols: 64 columns a workgroup, 16 slices of the rows, every load of a slice in flight
@@ -417,15 +417,23 @@ constexpr int kRegCols = 16384;
 int long_slices(int64_t rows) { return (int)std::max(std::min(rows, (int64_t)32), (rows + kChain - 1) / kChain); }
 
 // Workgroups of the backward pass: as many as run at once; each costs a partial row of 2 * cols floats, so wide rows get fewer (8192 x 8000 in
-// fp32: 116 us with 256, 126 with 512).  More only where one would make over kChain trips.
-int bwd_groups(int64_t rows, int cols) {
-  int64_t per = 1;
-  const int cap = cols <= 384 ? 1024 : cols <= 4096 ? 512 : 256;
+// fp32: 116 us with 256, 126 with 512).  Rows that would make over kChain trips are further launches, one behind the other: as more workgroups
+// in one launch they would be walked in strides that memory likes less (300000 x 4096 in bf16: 2310 -> 2630 us).
+struct BwdPlan { int cap, per; };        // workgroups of a launch at most, rows side by side in one
+BwdPlan bwd_plan(int cols) {
+  int per = 1;
 #define X(TPR, NCH, NT) if (cols <= TPR * NCH * 8 && per == 1 && NT / TPR > 1) per = NT / TPR;
   HCM_NORM_SHAPES(X)
 #undef X
-  const int64_t need = (rows + per - 1) / per;
-  return (int)std::max(std::min(need, (int64_t)cap), (need + kChain - 1) / kChain);
+  return {cols <= 384 ? 1024 : cols <= 4096 ? 512 : 256, per};
+}
+int64_t bwd_launch_rows(const BwdPlan& p) { return (int64_t)p.cap * p.per * kChain; }
+int bwd_groups(const BwdPlan& p, int64_t rows) { return (int)std::min((rows + p.per - 1) / p.per, (int64_t)p.cap); }
+// partial rows of all launches
+int bwd_parts(int64_t rows, int cols) {
+  const BwdPlan p = bwd_plan(cols);
+  const int64_t chunk = bwd_launch_rows(p);
+  return (int)(rows / chunk * p.cap + bwd_groups(p, rows % chunk));
 }
 
 template <typename T>
@@ -451,10 +459,17 @@ int bwd(const void* x, int64_t ldx, const uint8_t* q, int64_t ldq, const uint8_t
         const float* mean, const float* rstd, void* dx, float* part, int& parts, hipStream_t st) {
 #define X(TPR, NCH, NT)                                                                                                                            \
   if (cols <= TPR * NCH * 8) {                                                                                                                     \
-    parts = bwd_groups(rows, cols);                                                                                                                \
-    norm_bwd_kernel<T, ACT8, TPR, NCH, NT><<<parts, NT, 0, st>>>((const T*)x, ldx, q, ldq, scale, lds, (const T*)dy, (uint32_t)rows, cols, P, mean, rstd, \
-                                                                 (T*)dx, part);                                                                    \
-    HCM_CHECK_LAUNCH();                                                                                                                            \
+    const BwdPlan p = bwd_plan(cols);                                                                                                              \
+    parts = 0;                                                                                                                                     \
+    for (int64_t r = 0; r < rows; r += bwd_launch_rows(p)) {                                                                                       \
+      const int64_t n = std::min(rows - r, bwd_launch_rows(p));                                                                                    \
+      const int groups = bwd_groups(p, n);                                                                                                         \
+      norm_bwd_kernel<T, ACT8, TPR, NCH, NT><<<groups, NT, 0, st>>>(ACT8 ? nullptr : (const T*)x + r * ldx, ldx, ACT8 ? q + r * ldq : nullptr, ldq,\
+                                                                    ACT8 ? scale + r * lds : nullptr, lds, (const T*)dy + r * cols, (uint32_t)n, cols,\
+                                                                    P, mean + r, rstd + r, (T*)dx + r * cols, part + (int64_t)parts * 2 * cols);   \
+      HCM_CHECK_LAUNCH();                                                                                                                          \
+      parts += groups;                                                                                                                             \
+    }                                                                                                                                              \
     return 0;                                                                                                                                      \
   }
   HCM_NORM_SHAPES(X)
@@ -493,7 +508,7 @@ int hcm_layer_norm_forward(const void* x, int dtype, int64_t rows, int cols, int
 
 size_t hcm_layer_norm_backward_workspace_bytes(int64_t rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int64_t parts = cols > kRegCols ? long_slices(rows) : bwd_groups(rows, cols);
+  const int64_t parts = cols > kRegCols ? long_slices(rows) : bwd_parts(rows, cols);
   return (size_t)parts * 2 * cols * sizeof(float);
 }
 
