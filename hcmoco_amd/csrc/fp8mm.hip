@@ -460,32 +460,24 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s* lds_v4s;
 
 // Eight floats -> the bf16 pieces that hold their type exactly (down to bf16's smallest step, 2^-133: values under 2^-110 keep fewer
-// bits).  What would round up to bf16's infinity is rare and goes by itself: a finite value is cut off to bf16 first, and an
-// infinity has no remainder (inf - inf would make its NaN of it).
+// bits).  The first piece is cut off, not rounded: the remainder is as exact, and the largest finite values do not round up to infinity.  An
+// infinity has no remainder (inf - inf would make its products NaN).
 template <int P>
 __device__ __forceinline__ void pieces(const float (&v)[8], v8bf (&out)[P]) {
-  const float over = __uint_as_float(0x7f7f8000u);
-  float r[8], top = 0.f;
+  float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = v[i], top = fmaxf(top, fabsf(v[i]));
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) out[p][i] = (__bf16)r[i];
-    if (p == 0 && top >= over)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (fabsf(r[i]) >= over) {
-          out[0][i] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(r[i]) >> 16));
-          if (!finite_f(r[i])) r[i] = 0.f;
-          else r[i] -= (float)out[0][i];
-        } else {
-          r[i] -= (float)out[0][i];
-        }
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] -= (float)out[p][i];
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t cut = __float_as_uint(v[i]) & 0xffff0000u;
+    out[0][i] = __builtin_bit_cast(__bf16, (uint16_t)(cut >> 16));
+    r[i] = __builtin_isinf(v[i]) ? 0.f : v[i] - __uint_as_float(cut);
   }
+#pragma unroll
+  for (int p = 1; p < P; ++p)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      out[p][i] = (__bf16)r[i];
+      r[i] -= (float)out[p][i];
+    }
 }
 
 // TK columns k x TN columns n of dW a workgroup of WK x WN = 8 waves; ROWS rows m a stage, two stages.  What a stage needs is on its
