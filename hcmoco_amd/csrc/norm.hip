@@ -411,6 +411,7 @@ __global__ __launch_bounds__(256) void norm_long_cols_kernel(const T* __restrict
 #define HCM_NORM_SHAPES(X)                                                                                   \
   X(16, 1, 256) X(16, 3, 256) X(64, 1, 256) X(64, 2, 256) X(64, 4, 256) X(256, 2, 256) X(256, 4, 256) X(512, 4, 512)
 
+// what the widest shape holds; rows of 16385 walk memory (4096 rows of bf16, forward: 54 us at 16384 columns, 130 at 16385)
 constexpr int kRegCols = 16384;
 
 // slices of the rows in norm_long_cols_kernel
