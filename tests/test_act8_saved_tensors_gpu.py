@@ -110,3 +110,22 @@ def test_something_else_is_refused(wrong):
                 y = op(*leaves)
                 with pytest.raises(RuntimeError):
                     torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_under_activation_checkpointing(reentrant):
+    from hcmoco_amd import hip_ops
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(8)
+    wide = torch.randn(60, 333, generator=g).to(DEV)
+    p = [torch.randn(s, generator=g).to(DEV) for s in ((270,), (270,), (90, 270), (90,), (90,), (40, 90))]
+    dy = torch.randn(60, 40, generator=g).to(DEV)
+
+    def block(x, w1, b1, W1, B1, w2, W2):
+        h = hip_ops.fp8_linear(hip_ops.layer_norm(x, w1, b1), W1, B1)
+        return hip_ops.fp8_linear(hip_ops.layer_norm(h, w2, act8=True), W2)
+    leaves = [t.detach().requires_grad_() for t in [wide[:, 3:273]] + p]
+    want = _grads(block, leaves, dy)
+    y = checkpoint(block, *leaves, use_reentrant=reentrant)
+    y.backward(dy)
+    assert all(torch.equal(t.grad, q) for t, q in zip(leaves, want))

@@ -133,3 +133,33 @@ def test_many_rows_of_a_column_slice(rows, cols):
     want, err = _truth(x, w.detach(), b.detach(), dy, 1e-5)
     for g, t, e, n, d in zip(got, want, err, ('y', 'dx', 'dw', 'db'), (torch.bfloat16, torch.bfloat16, torch.float32, torch.float32)):
         _check(g, t.cpu(), e.cpu(), (n, d))
+
+
+@pytest.mark.parametrize('act8', [False, True])
+@pytest.mark.parametrize('rows,cols,dtype', [(4200007, 8, torch.float32), (2 * 4194304, 5, torch.bfloat16), (131077, 2049, torch.float16)])
+def test_more_rows_than_one_launch_takes(rows, cols, dtype, act8):
+    """256 rows of each workgroup of a launch (4194304 rows up to 384 columns, 131072 of 2049..4096), then the next launch: eager, and captured
+    and replayed.  The column sums: chains of 256 + 16 side by side + at most 2048 partial rows by 64 + 20 < 350, where _truth() has 66."""
+    from act8_ref import held8
+    from hcmoco_amd import hip_ops
+    from test_layer_norm_gpu import _check, _inputs, _run, _truth
+    x, w, b, dy = _inputs(rows, cols, dtype, cols)
+    x8 = held8(x)[0].to(DEV) if act8 else None
+    got = _run(x, w, b, dy, 1e-5, act8)
+    want, err = _truth(*(t.to(DEV) for t in (x, w, b, dy)), 1e-5, x8)
+    for g, t, e, n, d, long in zip(got, want, err, ('y', 'dx', 'dw', 'db'), (dtype, dtype, torch.float32, torch.float32), (1, 1, 6, 6)):
+        _check(g, t.cpu(), long * e.cpu(), (n, d))
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    dy = dy.to(DEV)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        y = hip_ops.layer_norm(*leaves, act8=act8)
+        outs = [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs, got))
